@@ -315,6 +315,136 @@ ZTVM_API int ztvm_moe_router_topk(ztvm_ctx* ctx, uint64_t out_idx, uint64_t out_
 ZTVM_API int ztvm_moe_slot_translate(ztvm_ctx* ctx, uint64_t ids_out, uint64_t ids_in, uint64_t slot_map, uint32_t n,
                                      uint32_t map_len);
 
+/* ---- verifying drafted tokens: the dispatches between the QKV matmul of several rows and the answer ----
+ * The entry points above write the paged cache for one token of one sequence. The four below do the step of
+ * several tokens (a prompt chunk, a chain or a tree of drafted tokens, a decode batch): rotate and store, attend,
+ * read back, score. The reference has the single-token forms of the first two as WGSL pipelines (rope.wgsl,
+ * kv_append.wgsl, attention*.wgsl); trees, batches and the scores are this library's. Every index that comes from
+ * device memory (positions, slots, page numbers, lengths) is checked in the kernel, so a bad one cannot fault the
+ * GPU; the descriptors are checked before anything is enqueued, and before the context is looked at, so that a
+ * descriptor can be tried with a null context on a machine without a GPU ("null context" is then the only
+ * complaint left). All may be recorded. */
+
+/* A paged cache as ztvm_qkv_fused (F16) or ztvm_kv_quantize_int8 (INT8) writes it. */
+enum {
+  ZTVM_KV_F16 = 0, /* element page*kv_page_stride + head*head_page_stride + slot*head_dim + dim (+ v_page_offset for V) */
+  ZTVM_KV_INT8 = 1 /* word page . head . slot . side(K, V) . dim/4, and one f16 scale page . head . slot . side */
+};
+typedef struct ztvm_kv_cache {
+  uint32_t format; /* ZTVM_KV_* */
+  uint32_t kv_heads, head_dim, page_size;
+  uint32_t kv_page_stride, head_page_stride, v_page_offset; /* f16 elements; F16 only */
+  uint32_t pages_offset;  /* where page 0 starts behind `pages`: f16 elements (F16) or u32 words (INT8) */
+  uint32_t scales_offset; /* f16 elements; INT8 only */
+  uint32_t reserved;
+  uint64_t pages_capacity;  /* what is behind `pages`, in f16 elements or u32 words; required. A page that does not lie */
+  uint64_t scales_capacity; /* whole inside both capacities is outside the cache: never read, never written. */
+  uint64_t pages;           /* 16-byte aligned */
+  uint64_t scales;          /* INT8 only, 4-byte aligned */
+} ztvm_kv_cache;
+
+/* Rotary positions and the append of K and V for `tokens` rows of a fused QKV projection (rope.wgsl + kv_append.wgsl
+ * for several tokens at once). A row of `qkv` is [Q | K | V] = (heads + 2*kv_heads)*head_dim f16 elements, rows
+ * qkv_stride apart; the rotated Q rows go to q_out (q_stride apart; q_out may be qkv itself with the same stride,
+ * any other overlap is refused), the rotated K and the V into slot slots[t] of the cache: page slots[t] / page_size.
+ * Pair j < rotary_dim/2 of a head, elements (j, j + rotary_dim/2) or, interleaved, (2j, 2j+1), is turned by the
+ * angle positions[t] * frequencies[j] and scaled by attn_factor; elements from rotary_dim on pass unchanged. The
+ * angle is reduced to one turn in 64 bits, so far positions lose nothing; products and sums are f32 and round once
+ * to f16. INT8: the f16-rounded row is quantised as ztvm_kv_quantize_int8 does, bit for bit. A slot that is
+ * negative or in a page outside the cache stores nothing (its Q row is still written): that is how rows that only
+ * pad a batch are marked. Two tokens of one call must not name the same slot. */
+typedef struct ztvm_rope_append_desc {
+  uint32_t tokens, heads;
+  uint32_t rotary_dim;  /* even, 2..head_dim */
+  uint32_t interleaved; /* 0 | 1 */
+  uint32_t qkv_stride, q_stride; /* f16 elements between token rows */
+  float attn_factor;    /* > 0; 1 unless the frequencies were stretched (ztvm_rope_frequencies returns it) */
+  uint32_t reserved;
+  uint64_t qkv, q_out;
+  uint64_t frequencies; /* f64 [rotary_dim/2], radians per position */
+  uint64_t positions;   /* i32 [tokens] */
+  uint64_t slots;       /* i32 [tokens] */
+  ztvm_kv_cache cache;
+} ztvm_rope_append_desc;
+ZTVM_API int ztvm_rope_append(ztvm_ctx* ctx, const ztvm_rope_append_desc* desc);
+
+/* The frequency table for ztvm_rope_append, on the host (upload it once, as weights are). Replaces the reference's
+ * table builders (src/compiler/model-spec.ts:668-740). f_j = theta^(-2j/rotary_dim), then
+ *   LINEAR    f_j / factor
+ *   PIECEWISE wavelengths 2 pi/f_j past original/low_freq_factor are stretched by `factor`, below
+ *             original/high_freq_factor kept, between them blended linearly in original/wavelength
+ *   YARN      f_j / factor and f_j blended by a ramp over j between the pairs that make beta_fast and beta_slow turns
+ *             within `original` positions; *attn_factor = 0.1 ln(factor) + 1
+ * (factor >= 1; the other kinds give attn_factor 1). low / high are low_freq_factor / high_freq_factor or beta_slow /
+ * beta_fast, low < high. Needs no GPU. */
+enum { ZTVM_ROPE_PLAIN = 0, ZTVM_ROPE_LINEAR = 1, ZTVM_ROPE_PIECEWISE = 2, ZTVM_ROPE_YARN = 3 };
+ZTVM_API int ztvm_rope_frequencies(uint32_t kind, uint32_t rotary_dim, double theta, double factor, double original, double low,
+                                   double high, double* frequencies, float* attn_factor);
+
+/* Rows of the cache read back as f16: k_out / v_out [tokens][out_stride], head h at element h*head_dim of its row
+ * (INT8: f16(q * scale), the product in f32). Either output may be 0. A slot that is negative or in a page outside
+ * the cache leaves its rows as they were. */
+typedef struct ztvm_kv_read_desc {
+  uint32_t tokens, out_stride;
+  uint64_t k_out, v_out;
+  uint64_t slots; /* i32 [tokens] */
+  ztvm_kv_cache cache;
+} ztvm_kv_read_desc;
+ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
+
+/* Attention of the query tokens of several sequences over their cached keys and values. Sequence b owns query rows
+ * query_start[b] .. query_start[b+1]-1 (n_b of them, none is allowed) and the kv_length[b] cached positions
+ * 0 .. kv_length[b]-1, whose last n_b are its own query tokens, stored before the call; position p lies in page
+ * page_table[b*page_table_stride + p/page_size], slot p % page_size (page_table 0, one sequence only: page p/page_size).
+ * With context = kv_length[b] - n_b, query token i sees position p < kv_length[b] where
+ *   tree_mask == 0:  p <= context + i                                    (a chain, a prompt chunk, one decoded token)
+ *   tree_mask:       p < context, or bit (p - context) of its mask_words 64-bit words is set        (a tree)
+ * and p's page is inside the cache. Query head h reads kv head h / (heads/kv_heads).
+ *   out[t,h] = sum_p softmax_p(scale * q[t,h].k[p]) * v[p],   lse[t,h] = ln sum_p exp(scale * q[t,h].k[p])
+ * Sums are f32, the probabilities enter the product as f16 (relative 2^-11 each), out rounds once to f16. A token that
+ * sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
+ * matter. Rows outside every sequence are left as they were.
+ * max_query and max_kv bound n_b and kv_length[b] (the lengths are read on the device, so a recorded step can be
+ * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen. Scratch
+ * for the joined partial results comes from the context and depends on the descriptor only. */
+typedef struct ztvm_attention_desc {
+  uint32_t tokens;    /* rows of q, out, lse and tree_mask */
+  uint32_t sequences, heads;
+  uint32_t max_query, max_kv;
+  uint32_t q_stride, out_stride; /* f16 elements between token rows; head h starts at element h*head_dim */
+  uint32_t page_table_stride;
+  uint32_t mask_words; /* 64-bit words per token of tree_mask; at least max_query / 64, rounded up */
+  float scale;         /* finite */
+  uint64_t q, out;
+  uint64_t lse;         /* f32 [tokens][heads], or 0 */
+  uint64_t query_start; /* i32 [sequences + 1], ascending */
+  uint64_t kv_length;   /* i32 [sequences] */
+  uint64_t page_table;  /* i32 [sequences][page_table_stride], or 0 */
+  uint64_t tree_mask;   /* u64 [tokens][mask_words], or 0 */
+  ztvm_kv_cache cache;
+} ztvm_attention_desc;
+ZTVM_API int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* desc);
+
+/* What a row of logits says: y = logits * inv_temperature (f32), lse = ln sum exp(y),
+ *   logprob[r] = y[tokens[r]] - lse   (a token outside the vocabulary: -inf)
+ *   entropy[r] = -sum p ln p, p = exp(y - lse)
+ *   top_ids / top_logprobs [r][top_k]: the top_k largest logits in descending order, ties to the lower id, and y - lse of each
+ * Any output may be 0 (tokens is read for logprob only). A logit of -inf has probability zero; a row with nothing else
+ * has log probabilities -inf and entropy 0. A NaN or +inf among the logits makes the row's log probabilities and
+ * entropy NaN; the ids still follow the order of the logits, NaN last. */
+typedef struct ztvm_token_logprobs_desc {
+  uint32_t rows, vocab;
+  uint32_t row_stride;    /* elements between rows of logits, >= vocab */
+  uint32_t logits_f16;    /* 0: f32 logits (out_f32 of the LM head), 1: f16 */
+  uint32_t top_k;         /* 0..min(vocab, 64) */
+  float inv_temperature;  /* > 0, finite */
+  uint64_t logits;
+  uint64_t tokens;        /* i32 [rows] */
+  uint64_t logprob, entropy;      /* f32 [rows] */
+  uint64_t top_ids, top_logprobs; /* u32 / f32 [rows][top_k] */
+} ztvm_token_logprobs_desc;
+ZTVM_API int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* desc);
+
 /* ---- load-time repack of MLX safetensors records (buildBuffer) -------------
  * The records are uploaded as they sit in the file (ztvm_upload); these calls
  * build the bound buffers from them in device memory. `overflow` is the device
@@ -347,8 +477,8 @@ ZTVM_API int ztvm_repack_dequant_split(ztvm_ctx* ctx, uint64_t dst, uint64_t wei
 
 /* ---- command buffers (createCommandEncoder / finish / queue.submit) ------ */
 
-/* Between begin and end, ztvm_matmul / ztvm_dequant / ztvm_fill / ztvm_copy and
- * the block dispatches above are recorded instead of run (src/zero-tvm/engine-core.ts:2565-2570 records a
+/* Between begin and end, ztvm_matmul / ztvm_dequant / ztvm_fill / ztvm_copy, the
+ * block dispatches and the verification dispatches above are recorded instead of run (src/zero-tvm/engine-core.ts:2565-2570 records a
  * whole token into one encoder). Uploads, downloads and syncs are rejected
  * while recording. */
 ZTVM_API int ztvm_record_begin(ztvm_ctx* ctx);

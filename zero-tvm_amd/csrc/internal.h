@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include "kv_cache.h"
 
 namespace ztvm {
 
@@ -96,6 +97,52 @@ hipError_t launch_kv_quantize_int8(void* pages_i8, void* scales, const void* k_s
                                    uint32_t pages_word_off, uint32_t scales_off, uint64_t pages_capacity_words, uint64_t scales_capacity,
                                    hipStream_t s);
 hipError_t launch_slot_translate(void* ids_out, const void* ids_in, const void* slot_map, uint32_t n, uint32_t map_len, hipStream_t s);
+
+// verifying drafted tokens over the paged cache (kv_ops.hip, attention.hip, logprobs.hip)
+struct RopeAppendArgs {
+  const _Float16* qkv;
+  _Float16* q_out;
+  const double* frequencies;
+  const int32_t* positions;
+  const int32_t* slots;
+  uint32_t tokens, heads, rotary_dim, interleaved, qkv_stride, q_stride;
+  float attn_factor;
+  KvView cache;
+};
+struct KvReadArgs {
+  _Float16* k_out;
+  _Float16* v_out;
+  const int32_t* slots;
+  uint32_t tokens, out_stride;
+  KvView cache;
+};
+struct AttentionArgs {
+  const _Float16* q;
+  _Float16* out;
+  float* lse;
+  const int32_t* query_start;
+  const int32_t* kv_length;
+  const int32_t* page_table;
+  const uint64_t* tree_mask;
+  uint32_t tokens, sequences, heads, max_query, max_kv, q_stride, out_stride, page_table_stride, mask_words;
+  float scale;
+  KvView cache;
+};
+struct LogprobsArgs {
+  const void* logits;
+  const int32_t* tokens;
+  float* logprob;
+  float* entropy;
+  uint32_t* top_ids;
+  float* top_logprobs;
+  uint32_t rows, vocab, row_stride, f16, top_k;
+  float inv_temperature;
+};
+hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
+hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s);
+size_t attention_scratch_bytes(const AttentionArgs& a);
+hipError_t launch_attention(const AttentionArgs& a, void* scratch, hipStream_t s);
+hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t s);
 
 // load-time repacking of checkpoint records (repack.hip); convert: 0 raw, 1 bf16->f16, 2 bf16->f32
 hipError_t launch_repack_convert(void* dst, const void* src, size_t src_bytes, int convert, uint32_t* counter, hipStream_t s);

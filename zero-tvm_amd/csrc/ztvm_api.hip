@@ -6,6 +6,7 @@
 #include "skinny.h"
 #include "scratch_pool.h"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -293,6 +294,77 @@ int scratch_for(ztvm_ctx* ctx, size_t need, void** out) {
   }
   *out = pool.data();
   return ZTVM_OK;
+}
+
+// Kernels go to the context's device whatever device the calling thread has current (torch and others move it).
+struct DeviceGuard {
+  int before = -1;
+  bool ok = true;
+  explicit DeviceGuard(int device) {
+    int cur = 0;
+    if (hipGetDevice(&cur) == hipSuccess && cur == device) return;
+    before = cur;
+    ok = hipSetDevice(device) == hipSuccess;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// The cache of the verification dispatches as byte strides, or why it cannot be one.
+int cache_view(const ztvm_kv_cache* c, KvView* v, char* why, size_t n) {
+  if (c->format != ZTVM_KV_F16 && c->format != ZTVM_KV_INT8) { why_set(why, n, "cache: unknown format %u", c->format); return ZTVM_E_INVALID; }
+  const bool i8 = c->format == ZTVM_KV_INT8;
+  if (!c->kv_heads || !c->head_dim || !c->page_size) { why_set(why, n, "cache: kv_heads, head_dim and page_size must be > 0"); return ZTVM_E_INVALID; }
+  if (c->head_dim > 512u) { why_set(why, n, "cache: head_dim %u > 512", c->head_dim); return ZTVM_E_UNSUPPORTED; }
+  if (c->kv_heads > 65535u || c->page_size >= (1u << 31)) { why_set(why, n, "cache: kv_heads=%u or page_size=%u too large", c->kv_heads, c->page_size); return ZTVM_E_INVALID; }
+  if (!c->pages || (i8 && !c->scales)) { why_set(why, n, "cache: null buffer"); return ZTVM_E_INVALID; }
+  if ((c->pages & 15u) || (i8 && (c->scales & 3u))) { why_set(why, n, "cache: misaligned buffer (pages 16, scales 4 bytes)"); return ZTVM_E_INVALID; }
+  if (!c->pages_capacity || (i8 && !c->scales_capacity)) { why_set(why, n, "cache: the capacities are required (they arm the kernels' page check)"); return ZTVM_E_INVALID; }
+  if (c->pages_capacity >= (1ull << 60) || c->scales_capacity >= (1ull << 60)) { why_set(why, n, "cache: capacity too large"); return ZTVM_E_INVALID; }
+  *v = KvView{};
+  v->kv_heads = c->kv_heads;
+  v->head_dim = c->head_dim;
+  v->page_size = c->page_size;
+  v->int8 = i8;
+  v->by_page = make_fast_div(c->page_size);
+  if (i8) {
+    if (c->head_dim & 3u) { why_set(why, n, "cache: an int8 head_dim must be a multiple of 4 (got %u)", c->head_dim); return ZTVM_E_INVALID; }
+    const uint64_t scales_page = 2ull * c->kv_heads * c->page_size, words_page = scales_page * (c->head_dim / 4u);
+    v->slot_bytes = 2u * c->head_dim;
+    v->side_bytes = c->head_dim;
+    v->head_bytes = (uint64_t)c->page_size * v->slot_bytes;
+    v->page_bytes = c->kv_heads * v->head_bytes;
+    v->pages = reinterpret_cast<char*>(c->pages) + 4ull * c->pages_offset;
+    v->scales = reinterpret_cast<uint16_t*>(c->scales) + c->scales_offset;
+    const uint32_t a = kv_whole_pages(c->pages_capacity, c->pages_offset, words_page, words_page);
+    const uint32_t b = kv_whole_pages(c->scales_capacity, c->scales_offset, scales_page, scales_page);
+    v->num_pages = a < b ? a : b;
+  } else {
+    if ((uint64_t)c->page_size * c->head_dim > c->head_page_stride || (uint64_t)c->kv_heads * c->head_page_stride > c->v_page_offset ||
+        (uint64_t)c->v_page_offset + (uint64_t)c->kv_heads * c->head_page_stride > c->kv_page_stride) {
+      why_set(why, n, "cache: page layout overlaps (page_size*head_dim <= head_page_stride, kv_heads*head_page_stride <= v_page_offset, v_page_offset + kv_heads*head_page_stride <= kv_page_stride)");
+      return ZTVM_E_INVALID;
+    }
+    v->slot_bytes = 2u * c->head_dim;
+    v->side_bytes = 2ull * c->v_page_offset;
+    v->head_bytes = 2ull * c->head_page_stride;
+    v->page_bytes = 2ull * c->kv_page_stride;
+    v->pages = reinterpret_cast<char*>(c->pages) + 2ull * c->pages_offset;
+    v->num_pages = kv_whole_pages(c->pages_capacity, c->pages_offset, c->kv_page_stride, (uint64_t)c->v_page_offset + (uint64_t)c->kv_heads * c->head_page_stride);
+  }
+  return ZTVM_OK;
+}
+
+// Whether [a, a + rows of a_width every a_stride] and the like at b share a byte other than by being the same array:
+// two column windows of one wider array (equal strides, columns apart) do not.
+bool rows_overlap(uint64_t a, uint64_t a_width, uint64_t a_stride, uint64_t b, uint64_t b_width, uint64_t b_stride, uint64_t rows) {
+  const uint64_t a_end = a + (rows - 1) * a_stride + a_width, b_end = b + (rows - 1) * b_stride + b_width;
+  if (a_end <= b || b_end <= a) return false;
+  if (a_stride != b_stride) return true;
+  const uint64_t lo = a < b ? a : b, hi = a < b ? b : a, lo_width = a < b ? a_width : b_width, hi_width = a < b ? b_width : a_width;
+  const uint64_t col = (hi - lo) % a_stride;
+  return !(col >= lo_width && col + hi_width <= a_stride);
 }
 
 struct Option {
@@ -739,6 +811,190 @@ int ztvm_moe_slot_translate(ztvm_ctx* ctx, uint64_t ids_out, uint64_t ids_in, ui
   if (!n) return ZTVM_OK;
   HIP_TRY(ctx, launch_slot_translate(reinterpret_cast<void*>(ids_out), reinterpret_cast<const void*>(ids_in),
                                      reinterpret_cast<const void*>(slot_map), n, map_len, ctx->stream));
+  return ZTVM_OK;
+}
+
+// ---- verifying drafted tokens over the paged cache ------------------------------------------
+
+int ztvm_rope_append(ztvm_ctx* ctx, const ztvm_rope_append_desc* d) {
+  if (!d) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: null descriptor");
+  char why[256];
+  RopeAppendArgs a{};
+  int rc = cache_view(&d->cache, &a.cache, why, sizeof why);
+  if (rc) return fail(ctx, rc, "ztvm_rope_append: %s", why);
+  const uint32_t dim = d->cache.head_dim;
+  if (dim & 1u) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: head_dim must be even (got %u)", dim);
+  if (!d->heads || d->heads > 65535u) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: heads must be 1..65535 (got %u)", d->heads);
+  if (!d->rotary_dim || (d->rotary_dim & 1u) || d->rotary_dim > dim)
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: rotary_dim must be even and 2..head_dim (got %u of %u)", d->rotary_dim, dim);
+  if (d->interleaved > 1) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: interleaved must be 0 or 1");
+  const uint64_t width = ((uint64_t)d->heads + 2ull * d->cache.kv_heads) * dim, q_width = (uint64_t)d->heads * dim;
+  if (d->qkv_stride < width || d->q_stride < q_width)
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: qkv_stride=%u or q_stride=%u is less than a row (%llu, %llu)", d->qkv_stride, d->q_stride,
+                (unsigned long long)width, (unsigned long long)q_width);
+  if (!(d->attn_factor > 0.f) || d->attn_factor > 3.0e38f) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: attn_factor must be > 0 and finite");
+  if (!d->qkv || !d->q_out || !d->frequencies || !d->positions || !d->slots) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: null buffer");
+  if (((d->qkv | d->q_out) & 1u) || (d->frequencies & 7u) || ((d->positions | d->slots) & 3u))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: misaligned buffer (qkv and q_out 2, frequencies 8, positions and slots 4 bytes)");
+  if (d->tokens >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: too many tokens (%u)", d->tokens);
+  const bool in_place = d->q_out == d->qkv && d->q_stride == d->qkv_stride;
+  if (d->tokens && !in_place && rows_overlap(d->qkv, 2 * width, 2ull * d->qkv_stride, d->q_out, 2 * q_width, 2ull * d->q_stride, d->tokens))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: q_out overlaps qkv (only q_out = qkv with the same stride is allowed)");
+  if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
+  if (!d->tokens) return ZTVM_OK;
+  a.qkv = reinterpret_cast<const _Float16*>(d->qkv);
+  a.q_out = reinterpret_cast<_Float16*>(d->q_out);
+  a.frequencies = reinterpret_cast<const double*>(d->frequencies);
+  a.positions = reinterpret_cast<const int32_t*>(d->positions);
+  a.slots = reinterpret_cast<const int32_t*>(d->slots);
+  a.tokens = d->tokens; a.heads = d->heads; a.rotary_dim = d->rotary_dim; a.interleaved = d->interleaved;
+  a.qkv_stride = d->qkv_stride; a.q_stride = d->q_stride; a.attn_factor = d->attn_factor;
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return fail(ctx, ZTVM_E_HIP, "ztvm_rope_append: hipSetDevice(%d) failed", ctx->device);
+  HIP_TRY(ctx, launch_rope_append(a, ctx->stream));
+  return ZTVM_OK;
+}
+
+int ztvm_rope_frequencies(uint32_t kind, uint32_t rotary_dim, double theta, double factor, double original, double low, double high,
+                          double* frequencies, float* attn_factor) {
+  if (kind > ZTVM_ROPE_YARN) return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: unknown kind %u", kind);
+  if (!rotary_dim || (rotary_dim & 1u) || rotary_dim > 512u)
+    return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: rotary_dim must be even and 2..512 (got %u)", rotary_dim);
+  if (!(theta > 1.0) || !std::isfinite(theta)) return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: theta must be > 1");
+  if (kind != ZTVM_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: factor must be >= 1");
+  if (kind >= ZTVM_ROPE_PIECEWISE && (!(original > 0.0) || !std::isfinite(original) || !(low > 0.0) || !(high > low) || !std::isfinite(high)))
+    return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: original > 0 and 0 < low < high are required");
+  if (!frequencies) return fail(nullptr, ZTVM_E_INVALID, "ztvm_rope_frequencies: null table");
+  const double two_pi = 6.283185307179586476925;
+  // yarn: the pair that makes `turns` turns within `original` positions
+  auto pair_of = [&](double turns) { return rotary_dim * std::log(original / (turns * two_pi)) / (2.0 * std::log(theta)); };
+  double from = 0.0, to = 1.0;
+  if (kind == ZTVM_ROPE_YARN) {
+    from = std::fmax(std::floor(pair_of(high)), 0.0);
+    to = std::fmin(std::ceil(pair_of(low)), rotary_dim - 1.0);
+    if (!(to - from >= 1e-3)) to = from + 1e-3;
+  }
+  for (uint32_t j = 0; j < rotary_dim / 2; j++) {
+    const double f = std::pow(theta, -2.0 * j / rotary_dim);
+    double out = f;
+    if (kind == ZTVM_ROPE_LINEAR) out = f / factor;
+    if (kind == ZTVM_ROPE_PIECEWISE) {
+      const double turns = original * f / two_pi;  // original / wavelength
+      const double keep = std::fmin(std::fmax((turns - low) / (high - low), 0.0), 1.0);
+      out = (1.0 - keep) * f / factor + keep * f;
+    }
+    if (kind == ZTVM_ROPE_YARN) {
+      const double stretch = std::fmin(std::fmax((j - from) / (to - from), 0.0), 1.0);
+      out = stretch * f / factor + (1.0 - stretch) * f;
+    }
+    frequencies[j] = out;
+  }
+  if (attn_factor) *attn_factor = kind == ZTVM_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+  return ZTVM_OK;
+}
+
+int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* d) {
+  if (!d) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: null descriptor");
+  char why[256];
+  KvReadArgs a{};
+  int rc = cache_view(&d->cache, &a.cache, why, sizeof why);
+  if (rc) return fail(ctx, rc, "ztvm_kv_read: %s", why);
+  const uint64_t width = (uint64_t)d->cache.kv_heads * d->cache.head_dim;
+  if (d->out_stride < width) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: out_stride=%u is less than a row (%llu)", d->out_stride, (unsigned long long)width);
+  if ((!d->k_out && !d->v_out) || !d->slots) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: null buffer");
+  if (((d->k_out | d->v_out) & 1u) || (d->slots & 3u)) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: misaligned buffer (outputs 2, slots 4 bytes)");
+  if (d->tokens >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: too many tokens (%u)", d->tokens);
+  if (d->tokens && d->k_out && d->v_out && rows_overlap(d->k_out, 2 * width, 2ull * d->out_stride, d->v_out, 2 * width, 2ull * d->out_stride, d->tokens))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: k_out and v_out overlap");
+  if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
+  if (!d->tokens) return ZTVM_OK;
+  a.k_out = reinterpret_cast<_Float16*>(d->k_out);
+  a.v_out = reinterpret_cast<_Float16*>(d->v_out);
+  a.slots = reinterpret_cast<const int32_t*>(d->slots);
+  a.tokens = d->tokens; a.out_stride = d->out_stride;
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return fail(ctx, ZTVM_E_HIP, "ztvm_kv_read: hipSetDevice(%d) failed", ctx->device);
+  HIP_TRY(ctx, launch_kv_read(a, ctx->stream));
+  return ZTVM_OK;
+}
+
+int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
+  if (!d) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: null descriptor");
+  char why[256];
+  AttentionArgs a{};
+  int rc = cache_view(&d->cache, &a.cache, why, sizeof why);
+  if (rc) return fail(ctx, rc, "ztvm_attention: %s", why);
+  if (!d->heads || d->heads > 65535u || d->heads % d->cache.kv_heads)
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: heads must be a multiple of kv_heads, at most 65535 (got %u of %u)", d->heads, d->cache.kv_heads);
+  const uint64_t width = (uint64_t)d->heads * d->cache.head_dim;
+  if (d->q_stride < width || d->out_stride < width)
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: q_stride=%u or out_stride=%u is less than a row (%llu)", d->q_stride, d->out_stride, (unsigned long long)width);
+  if (!std::isfinite(d->scale)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: scale must be finite");
+  if (!d->q || !d->out || !d->query_start || !d->kv_length) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: null buffer");
+  if (((d->q | d->out) & 1u) || ((d->lse | d->query_start | d->kv_length | d->page_table) & 3u) || (d->tree_mask & 7u))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: misaligned buffer (q and out 2, lse, query_start, kv_length and page_table 4, tree_mask 8 bytes)");
+  if (d->tokens >= (1u << 31) || d->max_query >= (1u << 30) || d->max_kv >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: tokens, max_query or max_kv too large");
+  if (d->sequences > 65535u) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: at most 65535 sequences per dispatch (got %u)", d->sequences);
+  if (d->page_table) {
+    if ((uint64_t)d->page_table_stride * d->cache.page_size < d->max_kv)
+      return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: page_table_stride=%u pages of %u do not hold max_kv=%u", d->page_table_stride, d->cache.page_size, d->max_kv);
+  } else if (d->sequences > 1) {
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: several sequences need a page_table");
+  }
+  if (d->tree_mask && 64ull * d->mask_words < d->max_query)
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: mask_words=%u hold less than max_query=%u bits", d->mask_words, d->max_query);
+  if (d->tokens && d->sequences && rows_overlap(d->q, 2 * width, 2ull * d->q_stride, d->out, 2 * width, 2ull * d->out_stride, d->tokens))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: out overlaps q");
+  if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
+  if (!d->tokens || !d->sequences || !d->max_query) return ZTVM_OK;
+  a.q = reinterpret_cast<const _Float16*>(d->q);
+  a.out = reinterpret_cast<_Float16*>(d->out);
+  a.lse = reinterpret_cast<float*>(d->lse);
+  a.query_start = reinterpret_cast<const int32_t*>(d->query_start);
+  a.kv_length = reinterpret_cast<const int32_t*>(d->kv_length);
+  a.page_table = reinterpret_cast<const int32_t*>(d->page_table);
+  a.tree_mask = reinterpret_cast<const uint64_t*>(d->tree_mask);
+  a.tokens = d->tokens; a.sequences = d->sequences; a.heads = d->heads; a.max_query = d->max_query; a.max_kv = d->max_kv;
+  a.q_stride = d->q_stride; a.out_stride = d->out_stride; a.page_table_stride = d->page_table_stride; a.mask_words = d->mask_words;
+  a.scale = d->scale;
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return fail(ctx, ZTVM_E_HIP, "ztvm_attention: hipSetDevice(%d) failed", ctx->device);
+  void* scratch = nullptr;
+  const size_t need = attention_scratch_bytes(a);
+  if (need) {
+    rc = scratch_for(ctx, need, &scratch);
+    if (rc) return rc;
+  }
+  HIP_TRY(ctx, launch_attention(a, scratch, ctx->stream));
+  return ZTVM_OK;
+}
+
+int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* d) {
+  if (!d) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: null descriptor");
+  if (!d->vocab || d->vocab >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: vocab must be 1..2^31-1 (got %u)", d->vocab);
+  if (d->row_stride < d->vocab) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: row_stride=%u is less than vocab=%u", d->row_stride, d->vocab);
+  if (d->logits_f16 > 1) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: logits_f16 must be 0 or 1");
+  if (d->top_k > 64u || d->top_k > d->vocab) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: top_k must be 0..min(vocab, 64) (got %u of %u)", d->top_k, d->vocab);
+  if (!(d->inv_temperature > 0.f) || !std::isfinite(d->inv_temperature)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: inv_temperature must be > 0 and finite");
+  if (!d->logits) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: null logits");
+  if (d->logprob && !d->tokens) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: logprob needs tokens");
+  if ((d->logits & (d->logits_f16 ? 1u : 3u)) || ((d->tokens | d->logprob | d->entropy | d->top_ids | d->top_logprobs) & 3u))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: misaligned buffer (logits to their type, the rest 4 bytes)");
+  if (d->rows >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: too many rows (%u)", d->rows);
+  if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
+  if (!d->rows) return ZTVM_OK;
+  LogprobsArgs a{};
+  a.logits = reinterpret_cast<const void*>(d->logits);
+  a.tokens = reinterpret_cast<const int32_t*>(d->tokens);
+  a.logprob = reinterpret_cast<float*>(d->logprob);
+  a.entropy = reinterpret_cast<float*>(d->entropy);
+  a.top_ids = reinterpret_cast<uint32_t*>(d->top_ids);
+  a.top_logprobs = reinterpret_cast<float*>(d->top_logprobs);
+  a.rows = d->rows; a.vocab = d->vocab; a.row_stride = d->row_stride; a.f16 = d->logits_f16; a.top_k = d->top_k;
+  a.inv_temperature = d->inv_temperature;
+  DeviceGuard g(ctx->device);
+  if (!g.ok) return fail(ctx, ZTVM_E_HIP, "ztvm_token_logprobs: hipSetDevice(%d) failed", ctx->device);
+  HIP_TRY(ctx, launch_logprobs(a, ctx->stream));
   return ZTVM_OK;
 }
 

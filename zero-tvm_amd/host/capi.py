@@ -22,9 +22,12 @@ EXPORTS = [
     "ztvm_event_create", "ztvm_event_destroy", "ztvm_event_record", "ztvm_event_elapsed_ms",
     "ztvm_set_option", "ztvm_get_option",
     "ztvm_silu_mul", "ztvm_moe_combine", "ztvm_moe_router_logits", "ztvm_moe_router_topk", "ztvm_moe_slot_translate",
+    "ztvm_rope_append", "ztvm_rope_frequencies", "ztvm_kv_read", "ztvm_attention", "ztvm_token_logprobs",
     "ztvm_repack_part", "ztvm_repack_permute_rows", "ztvm_repack_dequant_split",
 ]
 CONVERT_RAW, CONVERT_BF16_F16, CONVERT_BF16_F32 = 0, 1, 2
+KV_F16, KV_INT8 = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_PIECEWISE, ROPE_YARN = 0, 1, 2, 3
 EXPERTS_UNCHECKED = 0xFFFFFFFF  # ztvm_matmul_desc.experts: the caller vouches for every id
 
 
@@ -58,6 +61,41 @@ class KvQuantizeDesc(C.Structure):
         "kv_heads", "head_dim", "page_size", "tokens", "position_map_elem_offset", "pages_word_offset", "scales_elem_offset",
         "reserved")] + [(n, C.c_uint64) for n in (
             "pages_capacity_words", "scales_capacity", "k_slot", "v_slot", "pages_i8", "scales", "position_map")]
+
+
+class KvCache(C.Structure):
+    """Mirror of ztvm_kv_cache."""
+    _fields_ = [(n, C.c_uint32) for n in (
+        "format", "kv_heads", "head_dim", "page_size", "kv_page_stride", "head_page_stride", "v_page_offset", "pages_offset",
+        "scales_offset", "reserved")] + [(n, C.c_uint64) for n in ("pages_capacity", "scales_capacity", "pages", "scales")]
+
+
+class RopeAppendDesc(C.Structure):
+    """Mirror of ztvm_rope_append_desc."""
+    _fields_ = [(n, C.c_uint32) for n in ("tokens", "heads", "rotary_dim", "interleaved", "qkv_stride", "q_stride")] + [
+        ("attn_factor", C.c_float), ("reserved", C.c_uint32)] + [
+        (n, C.c_uint64) for n in ("qkv", "q_out", "frequencies", "positions", "slots")] + [("cache", KvCache)]
+
+
+class KvReadDesc(C.Structure):
+    """Mirror of ztvm_kv_read_desc."""
+    _fields_ = [("tokens", C.c_uint32), ("out_stride", C.c_uint32)] + [
+        (n, C.c_uint64) for n in ("k_out", "v_out", "slots")] + [("cache", KvCache)]
+
+
+class AttentionDesc(C.Structure):
+    """Mirror of ztvm_attention_desc."""
+    _fields_ = [(n, C.c_uint32) for n in (
+        "tokens", "sequences", "heads", "max_query", "max_kv", "q_stride", "out_stride", "page_table_stride", "mask_words")] + [
+        ("scale", C.c_float)] + [(n, C.c_uint64) for n in (
+            "q", "out", "lse", "query_start", "kv_length", "page_table", "tree_mask")] + [("cache", KvCache)]
+
+
+class TokenLogprobsDesc(C.Structure):
+    """Mirror of ztvm_token_logprobs_desc."""
+    _fields_ = [(n, C.c_uint32) for n in ("rows", "vocab", "row_stride", "logits_f16", "top_k")] + [
+        ("inv_temperature", C.c_float)] + [(n, C.c_uint64) for n in (
+            "logits", "tokens", "logprob", "entropy", "top_ids", "top_logprobs")]
 
 
 _lib = None
@@ -114,6 +152,11 @@ def load():
     L.ztvm_repack_part.argtypes = [vp, u64, u64, C.c_size_t, C.c_int, u64]
     L.ztvm_repack_permute_rows.argtypes = [vp, u64, u64, C.c_size_t, u32, C.POINTER(u32), u32]
     L.ztvm_repack_dequant_split.argtypes = [vp, u64, u64, u64, u64, u32, u32, u32, u32, u64]
+    L.ztvm_rope_append.argtypes = [vp, C.POINTER(RopeAppendDesc)]
+    L.ztvm_rope_frequencies.argtypes = [u32, u32] + [C.c_double] * 5 + [C.POINTER(C.c_double), C.POINTER(C.c_float)]
+    L.ztvm_kv_read.argtypes = [vp, C.POINTER(KvReadDesc)]
+    L.ztvm_attention.argtypes = [vp, C.POINTER(AttentionDesc)]
+    L.ztvm_token_logprobs.argtypes = [vp, C.POINTER(TokenLogprobsDesc)]
     _lib = L
     return L
 
@@ -132,6 +175,18 @@ def resolve(desc):
     if rc < 0:
         raise ZtvmError(rc, L.ztvm_last_error(None).decode())
     return rc
+
+
+def rope_frequencies(kind, rotary_dim, theta, factor=1.0, original=0.0, low=0.0, high=0.0):
+    """(f64 table [rotary_dim/2] for ztvm_rope_append, attn_factor); needs no GPU."""
+    import numpy as np
+    L = load()
+    out, factor_out = np.empty(max(rotary_dim // 2, 1), np.float64), C.c_float()
+    rc = L.ztvm_rope_frequencies(kind, rotary_dim, theta, factor, original, low, high,
+                                 out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(factor_out))
+    if rc:
+        raise ZtvmError(rc, L.ztvm_last_error(None).decode())
+    return out, factor_out.value
 
 
 class Context:
@@ -220,6 +275,18 @@ class Context:
 
     def kv_quantize_int8(self, desc):
         self._chk(self._L.ztvm_kv_quantize_int8(self._h, C.byref(desc)))
+
+    def rope_append(self, desc):
+        self._chk(self._L.ztvm_rope_append(self._h, C.byref(desc)))
+
+    def kv_read(self, desc):
+        self._chk(self._L.ztvm_kv_read(self._h, C.byref(desc)))
+
+    def attention(self, desc):
+        self._chk(self._L.ztvm_attention(self._h, C.byref(desc)))
+
+    def token_logprobs(self, desc):
+        self._chk(self._L.ztvm_token_logprobs(self._h, C.byref(desc)))
 
     def dequant(self, desc):
         self._chk(self._L.ztvm_dequant(self._h, C.byref(desc)))
