@@ -1,7 +1,10 @@
 // Attention of the query tokens of several sequences over the paged cache.
 #include "internal.h"
 #include "kv_cache.h"
+#include "mma.h"
 #include "quant.h"
+
+#include <algorithm>
 
 namespace ztvm {
 namespace {
@@ -119,13 +122,601 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
   if (tid == 0 && p.lse) p.lse[(size_t)t * p.heads + h] = m == -INFINITY ? -INFINITY : m + logf(total);
 }
 
+// ------------------------------------------------------------------------------- the matrix-core kernel ----
+// A workgroup takes one sequence, one kv head, ROWS = 16*QT*RW query rows (row = token * group + head of the group) and
+// one chunk of the keys. RW waves share keys and split the rows, KW waves share rows and split the keys.
+//
+//   S^T = K Q^T   v_mfma_f32_16x16x32: A = 16 keys x 32 dims straight from the staged rows, B = the query rows, kept in
+//                 registers. Lane (c = lane/16, j = lane%16) then holds query j, keys 4c..4c+3 of each 16-key tile.
+//   O^T += V^T P  B = the probabilities exactly where the first product left them: k index (c, e) means key
+//                 16*(e/4) + 4c + e%4. A = 16 dims x 32 keys with the same meaning, which is what the transposing LDS
+//                 reads deliver from rows of V as they lie in the cache (ds_read_b64_tr_b16 takes 4 keys x 16 dims a
+//                 group of 16 lanes, ds_read_b64_tr_b8 8 keys x 16 dims), so nothing is shuffled between the products.
+//
+// The running maximum is lazy: a row's reference value moves only when a score exceeds it by 2^THR, so most tiles need no
+// exchange between lanes and no rescaling. Probabilities are lifted by 2^LIFT before they round to f16, which keeps
+// small ones out of its subnormal range; int8 keys' scales multiply the scores, int8 values' scales the probabilities.
+//
+// Keys and values travel global -> LDS without passing registers, 32 keys a wave and stage, 16-byte chunks XOR-swizzled
+// so that neither kind of read meets bank conflicts. A page holds a multiple of 16 slots here, so 16 keys always lie in
+// one page and their addresses are one scalar base and a constant per lane.
+
+// chunk swizzles. A row of `KD` 64-byte units starts at bank slot 4*KD*row mod 16 (16 slots of 16 bytes): the XOR supplies
+// the row bits that the pitch does not.
+template <int KD>
+__device__ __forceinline__ constexpr uint32_t swz_k(uint32_t row) {
+  const uint32_t hi = row >> 4;  // tells rows 16 apart: the 8-bit transposing read takes rows r and r + 16 together
+  return KD % 4 == 0 ? (row & 15u) ^ (hi << 3) : KD % 2 == 0 ? ((row >> 1) & 7u) ^ (hi << 2) : ((row >> 2) & 3u) ^ (hi << 1);
+}
+template <int KD>
+__device__ __forceinline__ constexpr uint32_t swz_v(uint32_t row) {  // pairs of chunks over eight rows
+  return KD % 4 == 0 ? (row & 7u) << 1 : KD % 2 == 0 ? ((row >> 1) & 3u) << 1 : ((row >> 2) & 1u) << 1;
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+struct MfmaParams {
+  AttentionArgs a;
+  float* partial;   // [sequence][head][row of max_query tokens][split][dim], times 2^LIFT
+  float2* partial_ml;  // reference value (log2) and sum
+  uint32_t splits, chunk, group;
+  float scale_log2;  // |scale| * log2 e
+  uint32_t negate;   // scale < 0: the queries change sign
+};
+
+constexpr float NOTHING = -3.0e38f;  // a row's reference value before its first key
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// eight signed bytes -> eight f16, exactly: the byte with its sign bit flipped goes under 1024's exponent
+__device__ __forceinline__ h8 widen_i8(u32x2 w) {
+  const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u;
+  const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+  const h2 r0 = as_h2(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - bias;
+  const h2 r1 = as_h2(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - bias;
+  const h2 r2 = as_h2(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
+  const h2 r3 = as_h2(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
+  return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
+}
+
+// Which keys k0 .. k0+31 a query token sees: bit j. `limit`: the first position it cannot see in any case.
+__device__ __forceinline__ uint32_t visible_bits(int64_t k0, int64_t context, int64_t limit, const uint64_t* words, uint32_t mask_words) {
+  const int64_t left = limit - k0;
+  uint32_t bits = left <= 0 ? 0u : left >= 32 ? ~0u : (1u << left) - 1u;
+  if (words && bits) {
+    const int64_t rel = k0 - context;  // bit of the first key; below zero: history
+    uint32_t seen;
+    if (rel <= -32) {
+      seen = ~0u;
+    } else if (rel < 0) {
+      const uint32_t n = (uint32_t)-rel;
+      seen = (uint32_t)(words[0] << n) | ((1u << n) - 1u);
+    } else {
+      const uint64_t w = (uint64_t)rel >> 6;
+      const uint32_t b = (uint32_t)rel & 63u;
+      uint64_t v = w < mask_words ? words[w] >> b : 0ull;
+      if (b > 32u && w + 1 < mask_words) v |= words[w + 1] << (64u - b);
+      seen = (uint32_t)v;
+    }
+    bits &= seen;
+  }
+  return bits;
+}
+
+template <int KD, bool INT8, int QT, int RW, int KW>
+struct MfmaShape {
+  static constexpr int DIM = 32 * KD;
+  static constexpr int ROWS = 16 * QT * RW;
+  static constexpr int STAGES = RW == 1 ? 2 : 3;
+  static constexpr int PART = 32 * DIM * (INT8 ? 2 : 4);  // bytes of 32 keys: K then V (int8: rows of K | V)
+  static constexpr int SCALES = INT8 ? 32 * 4 : 0;
+  static constexpr int STAGE = KW * (PART + SCALES);
+  static constexpr int PITCH = DIM + 4;  // of the joined rows
+  static constexpr int JOIN = KW > 1 ? KW * ROWS * PITCH * 4 + KW * ROWS * 8 : 0;
+  static constexpr int LDS = std::max(STAGES * STAGE, JOIN);
+};
+
+template <int KD, bool INT8, int QT, int RW, int KW>
+__global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const MfmaParams p) {
+  using Shape = MfmaShape<KD, INT8, QT, RW, KW>;
+  constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, ST = Shape::STAGES;
+  constexpr float THR = INT8 ? 2.f : 6.f, LIFT = INT8 ? 16.f : 512.f;  // probabilities stay below 2^THR * LIFT (* 515, int8): f16's range
+  constexpr int MOVES = INT8 ? KD * 2 : KD * 4;     // transfers of 1 KiB that bring 32 keys
+  constexpr int DMA = (MOVES + RW - 1) / RW;        // of which a wave makes so many (the last one twice where they do not share evenly)
+  extern __shared__ __align__(16) char lds[];
+  const AttentionArgs& a = p.a;
+  const KvView& c = a.cache;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t rw = wave % RW, kw = wave / RW;
+  const uint32_t lc = lane >> 4, lj = lane & 15u;
+
+  uint32_t id = blockIdx.x;
+  const uint32_t h = id % c.kv_heads;
+  id /= c.kv_heads;
+  const uint32_t b = id % a.sequences, split = id / a.sequences;
+  const int32_t start = a.query_start[b];
+  const int64_t n = (int64_t)a.query_start[b + 1] - start;
+  // tokens of this sequence that exist and are asked for
+  const int64_t tokens = min(min(n, (int64_t)a.max_query), (int64_t)a.tokens - start);
+  const uint32_t row0 = blockIdx.y * ROWS;
+  if (start < 0 || tokens <= 0 || row0 >= tokens * p.group) return;
+  const uint32_t rows = (uint32_t)tokens * p.group;
+  const int32_t length = min(max(a.kv_length[b], 0), (int32_t)a.max_kv);
+  const int64_t context = length - n;
+  const bool tree = a.tree_mask != nullptr;
+  const uint32_t last_row = min(row0 + ROWS, rows) - 1;
+  const int64_t seen_by_all = tree ? context : context + row0 / p.group + 1;
+  const int64_t seen_by_any = tree ? length : context + last_row / p.group + 1;
+  const int32_t k_last = (int32_t)max(min(seen_by_any, (int64_t)length), (int64_t)0);
+  const int32_t full = (int32_t)max(min(seen_by_all, (int64_t)length), (int64_t)0);  // keys below: every row sees them
+  const uint32_t parts = max(1u, ((uint32_t)k_last + p.chunk - 1) / p.chunk);  // splits that have keys (one writes the empty rows)
+  if (split >= parts) return;
+  const int32_t k_begin = (int32_t)(split * p.chunk), k_end = min(k_last, k_begin + (int32_t)p.chunk);
+  const int32_t turns = (k_end - k_begin + 32 * KW - 1) / (32 * KW);
+
+  // ---- the query rows, as B operands
+  const uint32_t wave_row = row0 + rw * 16 * QT;
+  h8 q[QT][KD];
+  int64_t limit[QT];          // first position the lane's row cannot see
+  const uint64_t* words[QT];  // its token's mask
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const uint32_t row = wave_row + 16 * t + lj, i = row / p.group;
+    const bool there = row < rows;
+    const _Float16* src = a.q + (size_t)(start + (there ? i : 0u)) * a.q_stride + (size_t)(h * p.group + (there ? row - i * p.group : 0u)) * DIM;
+    limit[t] = there ? (tree ? (int64_t)length : min((int64_t)length, context + i + 1)) : 0;
+    words[t] = tree ? a.tree_mask + (size_t)(start + (there ? i : 0u)) * a.mask_words : nullptr;
+#pragma unroll
+    for (int s = 0; s < KD; s++) {
+      u32x4 v = *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * lc);
+      if (p.negate) v ^= 0x80008000u;
+      if (!there) v = u32x4{0, 0, 0, 0};
+      q[t][s] = __builtin_bit_cast(h8, v);
+    }
+  }
+
+  // ---- transfers: the lane's constant part of each address
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  // KD transfers move 16 rows of one side (f16) or of both (int8, K | V). Transfer g of the MOVES that bring 32 keys:
+  // f16: K of keys 0-15, of 16-31, then V; int8: keys 0-15, 16-31. A wave makes those of its turn among the RW.
+  uint32_t voff[DMA];
+#pragma unroll
+  for (int i = 0; i < DMA; i++) {
+    const uint32_t g = min((uint32_t)i * RW + rw, MOVES - 1u), within = g % (2 * KD);
+    const uint32_t idx = within * 64 + lane, row = idx / (4 * KD), ch = idx - row * (4 * KD);
+    const uint32_t swz = INT8 || g < 2 * KD ? swz_k<KD>(row) : swz_v<KD>(row);
+    voff[i] = (row & 15u) * c.slot_bytes + ((ch ^ swz) * 16);
+  }
+  const char* head_base = c.pages + (uint64_t)h * c.head_bytes;
+  auto base_of = [&](int32_t pos, bool& valid) -> const char* {  // 16 keys from pos on; uniform
+    uint32_t page = 0, slot = 0;
+    valid = pos < k_end;
+    if (valid) {
+      const uint32_t pno = fast_div(c.by_page, (uint32_t)pos);
+      slot = (uint32_t)pos - pno * c.page_size;
+      page = a.page_table ? (uint32_t)a.page_table[(size_t)b * a.page_table_stride + pno] : pno;
+      valid = page < c.num_pages;
+    }
+    if (!valid) page = slot = 0;  // some rows that exist; nobody sees them
+    return head_base + (uint64_t)page * c.page_bytes + (uint64_t)slot * c.slot_bytes;
+  };
+  auto scales_of = [&](int32_t pos) -> const char* {
+    uint32_t page = 0, slot = 0;
+    if (pos < k_end) {
+      const uint32_t pno = fast_div(c.by_page, (uint32_t)pos);
+      slot = (uint32_t)pos - pno * c.page_size;
+      page = a.page_table ? (uint32_t)a.page_table[(size_t)b * a.page_table_stride + pno] : pno;
+      if (page >= c.num_pages) page = slot = 0;
+    }
+    return reinterpret_cast<const char*>(c.scales + kv_scale_index(c, page, h, slot, 0));
+  };
+  auto issue = [&](int32_t turn, uint32_t stage) {
+    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
+    const uint32_t at = lds_base + stage * Shape::STAGE + kw * Shape::PART;
+    bool ok0, ok1;
+    const char* base0 = base_of(pos, ok0);
+    const char* base1 = base_of(pos + 16, ok1);
+    static_for<DMA>([&](auto i_) {
+      constexpr int i = decltype(i_)::value;
+      const uint32_t g = min((uint32_t)i * RW + rw, MOVES - 1u);
+      const char* base = g / KD % 2 ? base1 : base0;
+      if (!INT8 && g >= 2 * KD) base += c.side_bytes;
+      dma16<0>(base, voff[i], at + 1024u * g);
+    });
+  };
+  // int8 scales of the wave's 32 keys, K | V per key: lane j < 32 holds key j's pair
+  auto fetch_scales = [&](int32_t turn) -> uint32_t {
+    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
+    const char* s0 = scales_of(pos);
+    const char* s1 = scales_of(pos + 16);
+    const char* s = lane & 16u ? s1 : s0;
+    return *reinterpret_cast<const uint32_t*>(s + 4u * lj);
+  };
+
+  f4 acc[QT][2 * KD];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    m[t] = NOTHING;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 2 * KD; d++) acc[t][d] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto compute = [&](int32_t turn, uint32_t stage, uint32_t scale_pair) {
+    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
+    if (pos >= k_end) return;
+    const char* kv = lds + stage * Shape::STAGE + kw * Shape::PART;
+    f4 s[QT][2];
+#pragma unroll
+    for (int t = 0; t < QT; t++) s[t][0] = s[t][1] = f4{0.f, 0.f, 0.f, 0.f};
+    static_for<2>([&](auto half_) {
+      constexpr int half = decltype(half_)::value;
+      const uint32_t row = 16 * half + lj;
+#pragma unroll
+      for (int x = 0; x < KD; x++) {
+        h8 k;
+        if constexpr (INT8) {  // 8 bytes: half of a chunk
+          const uint32_t ch = 2 * x + (lc >> 1);
+          k = widen_i8(*reinterpret_cast<const u32x2*>(kv + row * (2 * DIM) + ((ch ^ swz_k<KD>(row)) * 16) + (lc & 1u) * 8));
+        } else {
+          k = *reinterpret_cast<const h8*>(kv + row * (2 * DIM) + (((4 * x + lc) ^ swz_k<KD>(row)) * 16));
+        }
+#pragma unroll
+        for (int t = 0; t < QT; t++) s[t][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[t][x], s[t][half], 0, 0, 0);
+      }
+    });
+    // scales: log2 units of the scores, and what the values' rows weigh
+    float ks[2][4], vs[2][4];
+    if constexpr (INT8) {
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const h2 pair = as_h2(__builtin_amdgcn_ds_bpermute((int)(4u * (16 * half + 4 * lc + i)), (int)scale_pair));
+          ks[half][i] = (float)pair.x * p.scale_log2;
+          vs[half][i] = (float)pair.y * LIFT;
+        }
+    }
+    bool edge = pos + 32 > full;
+    bool ok0 = true, ok1 = true;
+    if (!edge) {
+      base_of(pos, ok0);
+      base_of(pos + 16, ok1);
+      edge = !(ok0 && ok1);
+    }
+    h8 pf[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      float x[2][4];
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[half][i] = s[t][half][i] * (INT8 ? ks[half][i] : p.scale_log2);
+      uint32_t seen = ~0u;
+      if (edge) {
+        base_of(pos, ok0);
+        base_of(pos + 16, ok1);
+        seen = visible_bits(pos, context, limit[t], words[t], a.mask_words) & (ok0 ? ~0u : 0xFFFF0000u) & (ok1 ? ~0u : 0x0000FFFFu);
+        seen >>= 4 * lc;
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[half][i] = seen >> (16 * half + i) & 1u ? x[half][i] : -INFINITY;
+      }
+      float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+      if (__any(most > m[t] + THR)) {
+        const float next = fmaxf(m[t], across_groups_max(most));
+        const float keep = __builtin_amdgcn_exp2f(m[t] - next);
+        m[t] = next;
+        l[t] *= keep;
+#pragma unroll
+        for (int d = 0; d < 2 * KD; d++) acc[t][d] *= keep;
+      }
+#pragma unroll
+      for (int half = 0; half < 2; half++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float e = __builtin_amdgcn_exp2f(x[half][i] - m[t]);
+          l[t] += e;
+          float w = e * (INT8 ? vs[half][i] : LIFT);
+          if (INT8 && edge) w = seen >> (16 * half + i) & 1u ? w : 0.f;  // a scale nobody wrote may be anything
+          pf[t][4 * half + i] = (_Float16)w;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < 2 * KD; d++) {
+      h8 v;
+      if constexpr (INT8) {
+        const uint32_t row = 16 * (lj >> 3) + 4 * lc + ((lj >> 1) & 3u), ch = 2 * KD + d;
+        const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(kv + row * (2 * DIM) + ((ch ^ swz_k<KD>(row)) * 16) + (lj & 1u) * 8));
+        v = widen_i8(u32x2{(uint32_t)raw.x, (uint32_t)raw.y});
+      } else {
+        const uint32_t ch = 2 * d + ((lj & 3u) >> 1);
+        s16x4 r[2];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const uint32_t row = 16 * half + 4 * lc + (lj >> 2);
+          r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(kv + 64 * DIM + row * (2 * DIM) + ((ch ^ swz_v<KD>(row)) * 16) + (lj & 1u) * 8));
+        }
+        v = __builtin_bit_cast(h8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        if (edge) {
+          // An infinity or NaN that nobody sees must not enter as 0 * inf: the product gets a zero, and rows that do
+          // see it get it back by its sign.
+          u16x8 bits = __builtin_bit_cast(u16x8, v);
+          h8 up, down;
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint32_t e = bits[i];
+            const bool bad = (e & 0x7C00u) == 0x7C00u, nan = (e & 0x3FFu) != 0;
+            up[i] = bad && (nan || !(e & 0x8000u)) ? (_Float16)1.f : (_Float16)0.f;
+            down[i] = bad && (nan || (e & 0x8000u)) ? (_Float16)1.f : (_Float16)0.f;
+            bits[i] = bad ? 0 : e;
+            odd |= bad;
+          }
+          v = __builtin_bit_cast(h8, bits);
+          if (__any(odd)) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+              h8 sees;
+#pragma unroll
+              for (int i = 0; i < 8; i++) sees[i] = pf[t][i] > (_Float16)0.f ? (_Float16)1.f : (_Float16)0.f;
+              const f4 zero = {0.f, 0.f, 0.f, 0.f};
+              const f4 ups = __builtin_amdgcn_mfma_f32_16x16x32_f16(up, sees, zero, 0, 0, 0);
+              const f4 downs = __builtin_amdgcn_mfma_f32_16x16x32_f16(down, sees, zero, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (ups[i] > 0.f) acc[t][d][i] += INFINITY;
+                if (downs[i] > 0.f) acc[t][d][i] -= INFINITY;
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < QT; t++) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[t], acc[t][d], 0, 0, 0);
+    }
+  };
+
+  // ---- the pipeline
+  if constexpr (RW == 1) {  // a wave's keys are its own: no barrier
+#pragma unroll
+    for (int i = 0; i < ST; i++)
+      if (i < turns) issue(i, i);
+    for (int32_t turn = 0; turn < turns; turn++) {
+      const uint32_t stage = turn % ST;
+      uint32_t pair_now = 0;
+      if constexpr (INT8) pair_now = fetch_scales(turn);
+      if (turn + 1 < turns) wait_vm<(ST - 1) * DMA>();
+      else wait_vm<0>();
+      compute(turn, stage, pair_now);
+      wait_lgkm<0>();
+      if (turn + ST < turns) issue(turn + ST, stage);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++)
+      if (i < turns) issue(i, i);
+    for (int32_t turn = 0; turn < turns; turn++) {
+      uint32_t pair_now = 0;
+      if constexpr (INT8) pair_now = fetch_scales(turn);
+      if (turn + 1 < turns) wait_vm<(ST - 2) * DMA>();
+      else wait_vm<0>();
+      wg_barrier();  // everybody's transfers of this stage have landed, everybody has left the stage before
+      if (turn + ST - 1 < turns) issue(turn + ST - 1, (turn + ST - 1) % ST);
+      compute(turn, turn % ST, pair_now);
+      wait_lgkm<0>();
+    }
+  }
+
+  // ---- join the key waves, then either the result or a partial one
+#pragma unroll
+  for (int t = 0; t < QT; t++) l[t] = across_groups_sum(l[t]);
+  const bool last = parts == 1;
+  auto store4 = [&](uint32_t row, uint32_t d, f4 v, float total) {  // four dims of a row; v is times LIFT
+    if (last) {
+      const uint32_t i = row / p.group;
+      const float inv = total > 0.f || total != total ? 1.0f / (total * LIFT) : 0.f;
+      h4 o;
+#pragma unroll
+      for (int x = 0; x < 4; x++) o[x] = narrow_f32(v[x] * inv);
+      *reinterpret_cast<h4*>(a.out + (size_t)(start + i) * a.out_stride + (size_t)(h * p.group + (row - i * p.group)) * DIM + d) = o;
+    } else {
+      const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits + split;
+      *reinterpret_cast<f4*>(p.partial + at * DIM + d) = v;
+    }
+  };
+  auto store_row = [&](uint32_t row, float top, float total) {
+    if (last) {
+      const uint32_t i = row / p.group;
+      if (a.lse) a.lse[(size_t)(start + i) * a.heads + h * p.group + (row - i * p.group)] = total > 0.f || total != total ? (top + __log2f(total)) * 0.69314718055994531f : -INFINITY;
+    } else {
+      const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits + split;
+      p.partial_ml[at] = make_float2(top, total);
+    }
+  };
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      const uint32_t row = wave_row + 16 * t + lj;
+      if (row < rows) {
+        if (lc == 0) store_row(row, m[t], l[t]);
+#pragma unroll
+        for (int d = 0; d < 2 * KD; d++) store4(row, 16 * d + 4 * lc, acc[t][d], l[t]);
+      }
+    }
+  } else {
+    float* joined = reinterpret_cast<float*>(lds);
+    float2* ml = reinterpret_cast<float2*>(lds + KW * ROWS * Shape::PITCH * 4);
+    __syncthreads();  // the stages are done with
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+      if (lc == 0) ml[kw * ROWS + rw * 16 * QT + 16 * t + lj] = make_float2(m[t], l[t]);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      const uint32_t local = rw * 16 * QT + 16 * t + lj;
+      float top = m[t];
+#pragma unroll
+      for (int k = 0; k < KW; k++) top = fmaxf(top, ml[k * ROWS + local].x);
+      const float keep = __builtin_amdgcn_exp2f(m[t] - top);
+#pragma unroll
+      for (int d = 0; d < 2 * KD; d++) *reinterpret_cast<f4*>(joined + (kw * ROWS + local) * Shape::PITCH + 16 * d + 4 * lc) = acc[t][d] * keep;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < ROWS * (DIM / 4); i += 64 * RW * KW) {
+      const uint32_t local = i / (DIM / 4), d = (i - local * (DIM / 4)) * 4, row = row0 + local;
+      if (row >= rows) continue;
+      float top = ml[local].x, total = 0.f;
+#pragma unroll
+      for (int k = 1; k < KW; k++) top = fmaxf(top, ml[k * ROWS + local].x);
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KW; k++) {
+        total += ml[k * ROWS + local].y * __builtin_amdgcn_exp2f(ml[k * ROWS + local].x - top);
+        v += *reinterpret_cast<const f4*>(joined + (k * ROWS + local) * Shape::PITCH + d);
+      }
+      store4(row, d, v, total);
+      if (d == 0) store_row(row, top, total);
+    }
+  }
+}
+
+// Adds the partial results of a row's splits, in their order. One wave per query row and head.
+__global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t rows_per_wg, uint32_t causal_rows, float lift) {
+  const AttentionArgs& a = p.a;
+  const KvView& c = a.cache;
+  const uint32_t lane = threadIdx.x & 63u, b = blockIdx.y;
+  const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 6);  // (row, kv head)
+  const uint32_t row = unit / c.kv_heads, h = unit - row * c.kv_heads;
+  const int32_t start = a.query_start[b];
+  const int64_t n = (int64_t)a.query_start[b + 1] - start;
+  const int64_t tokens = min(min(n, (int64_t)a.max_query), (int64_t)a.tokens - start);
+  if (start < 0 || tokens <= 0 || row >= tokens * p.group) return;
+  const int32_t length = min(max(a.kv_length[b], 0), (int32_t)a.max_kv);
+  const int64_t context = length - n;
+  // how many splits the row's workgroup had, as it worked it out
+  const uint32_t last_row = min(row / causal_rows * causal_rows + causal_rows, (uint32_t)tokens * p.group) - 1;
+  const int64_t seen_by_any = a.tree_mask ? length : context + last_row / p.group + 1;
+  const int32_t k_last = (int32_t)max(min(seen_by_any, (int64_t)length), (int64_t)0);
+  const uint32_t parts = max(1u, ((uint32_t)k_last + p.chunk - 1) / p.chunk);
+  if (parts == 1) return;
+  const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits;
+  float top = NOTHING;
+  for (uint32_t s = lane; s < parts; s += 64u) top = fmaxf(top, p.partial_ml[at + s].x);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float total = 0.f;
+  for (uint32_t s = lane; s < parts; s += 64u) total += p.partial_ml[at + s].y * __builtin_amdgcn_exp2f(p.partial_ml[at + s].x - top);
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+  const float inv = total > 0.f || total != total ? 1.0f / (total * lift) : 0.f;
+  const uint32_t i = row / p.group, head = h * p.group + (row - i * p.group);
+  _Float16* out = a.out + (size_t)(start + i) * a.out_stride + (size_t)head * c.head_dim;
+  for (uint32_t d = lane; d < c.head_dim; d += 64u) {
+    float v = 0.f;
+    for (uint32_t s = 0; s < parts; s++) v += p.partial[(at + s) * c.head_dim + d] * __builtin_amdgcn_exp2f(p.partial_ml[at + s].x - top);
+    out[d] = narrow_f32(v * inv);
+  }
+  if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top + __log2f(total)) * 0.69314718055994531f : -INFINITY;
+}
+
+// What the matrix-core kernel takes: whole 64-byte units of a head, pages of whole 16-key blocks, 16-byte rows.
+bool mfma_takes(const AttentionArgs& a) {
+  const KvView& c = a.cache;
+  const uint32_t kd = c.head_dim / 32;
+  if (c.head_dim % 32 || !(kd == 2 || kd == 3 || kd == 4 || kd == 8)) return false;
+  if (c.page_size % 16 || !c.num_pages || !a.max_kv) return false;
+  const uint64_t at = reinterpret_cast<uint64_t>(c.pages) | c.page_bytes | c.head_bytes | c.side_bytes | c.slot_bytes;
+  if (at % 16 || reinterpret_cast<uint64_t>(c.scales) % 4) return false;
+  if ((reinterpret_cast<uint64_t>(a.q) | reinterpret_cast<uint64_t>(a.out)) & 15u || a.q_stride % 8 || a.out_stride % 8) return false;
+  // the grid, and key positions a few turns past the last one, stay inside 31 bits
+  const uint64_t rows = (uint64_t)std::min(a.max_query, a.tokens) * a.heads;
+  return rows < (1u << 20) && a.max_kv < (1u << 30) && (uint64_t)a.sequences * c.kv_heads < (1u << 20);
+}
+
+struct MfmaPlan {
+  int qt, rw, kw;
+  uint32_t rows, row_tiles, splits, chunk;
+  size_t partial_bytes, bytes;
+};
+MfmaPlan mfma_plan(const AttentionArgs& a) {
+  MfmaPlan g{};
+  const uint32_t group = a.heads / a.cache.kv_heads;
+  const uint64_t rows = (uint64_t)std::min(a.max_query, a.tokens) * group;
+  const bool wide = a.cache.head_dim > 128;
+  if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = wide ? 2 : 4;
+  else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
+  else g.qt = 2, g.rw = 4, g.kw = 1;
+  g.rows = 16 * g.qt * g.rw;
+  g.row_tiles = (uint32_t)((rows + g.rows - 1) / g.rows);
+  const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
+  // enough workgroups for a few rounds of the CUs, none with less than four turns of its waves
+  const uint64_t want = 1024;
+  const uint32_t least = 32u * g.kw * 4u;
+  uint64_t splits = (want + groups - 1) / groups;
+  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (a.max_kv + least - 1) / least));
+  g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + 32 * g.kw - 1) / (32 * g.kw) * (32 * g.kw));
+  g.splits = (a.max_kv + g.chunk - 1) / g.chunk;
+  if (g.splits > 1) {
+    const uint64_t n = (uint64_t)a.sequences * a.heads * a.max_query * g.splits;
+    g.partial_bytes = n * a.cache.head_dim * 4;
+    g.bytes = g.partial_bytes + n * 8;
+  }
+  return g;
+}
+
+template <int KD, bool INT8, int QT, int RW, int KW>
+hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t s) {
+  using Shape = MfmaShape<KD, INT8, QT, RW, KW>;
+  auto kernel = attention_mfma_kernel<KD, INT8, QT, RW, KW>;
+  if (Shape::LDS > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
+  const dim3 grid(p.a.sequences * p.a.cache.kv_heads * g.splits, g.row_tiles);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * RW * KW), Shape::LDS, s, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || g.splits == 1) return e;
+  const uint32_t units = std::min(p.a.max_query, p.a.tokens) * p.a.heads;
+  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, 0u, (uint32_t)g.rows, INT8 ? 16.f : 512.f);
+  return hipGetLastError();
+}
+template <int KD, bool INT8>
+hipError_t launch_mfma_dim(const MfmaParams& p, const MfmaPlan& g, hipStream_t s) {
+  constexpr int KW = KD > 4 ? 2 : 4;
+  if (g.rw == 4) return launch_mfma_shape<KD, INT8, 2, 4, 1>(p, g, s);
+  if (g.qt == 2) return launch_mfma_shape<KD, INT8, 2, 1, KW>(p, g, s);
+  return launch_mfma_shape<KD, INT8, 1, 1, KW>(p, g, s);
+}
+
 }  // namespace
 
-size_t attention_scratch_bytes(const AttentionArgs&) { return 0; }
+size_t attention_scratch_bytes(const AttentionArgs& a) { return mfma_takes(a) ? mfma_plan(a).bytes : 0; }
 
-hipError_t launch_attention(const AttentionArgs& a, void*, hipStream_t s) {
-  hipLaunchKernelGGL(attention_any_kernel, dim3(a.tokens, a.heads), dim3(256), 0, s, a);
-  return hipGetLastError();
+hipError_t launch_attention(const AttentionArgs& a, void* scratch, hipStream_t s) {
+  if (!mfma_takes(a)) {
+    hipLaunchKernelGGL(attention_any_kernel, dim3(a.tokens, a.heads), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  const MfmaPlan g = mfma_plan(a);
+  MfmaParams p{a, static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + g.partial_bytes), g.splits, g.chunk,
+               a.heads / a.cache.kv_heads, fabsf(a.scale) * 1.4426950408889634f, a.scale < 0.f};
+  auto by_format = [&](auto kd) {
+    constexpr int KD = decltype(kd)::value;
+    return a.cache.int8 ? launch_mfma_dim<KD, true>(p, g, s) : launch_mfma_dim<KD, false>(p, g, s);
+  };
+  switch (a.cache.head_dim / 32) {
+    case 2: return by_format(ic<2>{});
+    case 3: return by_format(ic<3>{});
+    case 4: return by_format(ic<4>{});
+    default: return by_format(ic<8>{});
+  }
 }
 
 }  // namespace ztvm
