@@ -437,7 +437,7 @@ typedef struct ztvm_token_logprobs_desc {
   uint32_t row_stride;    /* elements between rows of logits, >= vocab */
   uint32_t logits_f16;    /* 0: f32 logits (out_f32 of the LM head), 1: f16 */
   uint32_t top_k;         /* 0..min(vocab, 64) */
-  float inv_temperature;  /* > 0, finite */
+  float inv_temperature;  /* > 0, at most 1e38 */
   uint64_t logits;
   uint64_t tokens;        /* i32 [rows] */
   uint64_t logprob, entropy;      /* f32 [rows] */

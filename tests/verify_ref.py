@@ -94,10 +94,10 @@ def attention(q, rows, page, table, starts, lengths, masks, scale, heads):
 def close_attention(got, got_lse, want, lse, weight, slack, total, dim, keys):
     """f32 dot products of `dim` terms are off by (dim + 4) 2^-23 of the sum of their magnitudes, which moves a probability
     by twice that; each probability rounds to f16 once (2^-11), the running sums and exponentials add under 2^-18. A
-    probability near f16's smallest step is off by at most 2^-25 of it, times 127 counts, over the lift of 64: keys *
-    2^-24 over the sum of the probabilities. The result rounds to f16 once."""
+    probability near f16's smallest step is off by at most 2^-25, which 127 counts multiply and the lift of 16 that int8
+    probabilities enter with divides: under keys * 2^-22 over the sum of the probabilities. The result rounds to f16 once."""
     score = slack * (dim + 4) * 2.0 ** -23
-    bound = HALF * np.abs(want) + TINY / 2 + weight * (HALF + 2 * score[..., None] + 2.0 ** -18) + keys * TINY / total[..., None]
+    bound = HALF * np.abs(want) + TINY / 2 + weight * (HALF + 2 * score[..., None] + 2.0 ** -18) + keys * 4 * TINY / total[..., None]
     got = np.asarray(got, np.float64)
     assert np.all(np.isfinite(got)), "non-finite output"
     assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) / bound))

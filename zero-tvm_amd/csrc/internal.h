@@ -142,7 +142,8 @@ hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
 hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s);
 size_t attention_scratch_bytes(const AttentionArgs& a);
 hipError_t launch_attention(const AttentionArgs& a, void* scratch, hipStream_t s);
-hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t s);
+size_t logprobs_scratch_bytes(const LogprobsArgs& a);
+hipError_t launch_logprobs(const LogprobsArgs& a, void* scratch, hipStream_t s);
 
 // load-time repacking of checkpoint records (repack.hip); convert: 0 raw, 1 bf16->f16, 2 bf16->f32
 hipError_t launch_repack_convert(void* dst, const void* src, size_t src_bytes, int convert, uint32_t* counter, hipStream_t s);

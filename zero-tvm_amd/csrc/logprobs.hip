@@ -11,9 +11,10 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   return v != v ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u);
 }
 
-// One workgroup per row, one pass for the maximum, one for the sums, one for each alternative.
+// Rows too long for the table of neighbourhoods below: one workgroup per row, one pass for the maximum, one for the
+// sums, one for each alternative.
 template <class T>
-__global__ __launch_bounds__(256) void logprobs_kernel(const LogprobsArgs p) {
+__global__ __launch_bounds__(256) void logprobs_any_kernel(const LogprobsArgs p) {
   __shared__ float red[256];
   __shared__ unsigned long long best[256];
   const uint32_t r = blockIdx.x, tid = threadIdx.x;
@@ -86,12 +87,328 @@ __global__ __launch_bounds__(256) void logprobs_kernel(const LogprobsArgs p) {
   }
 }
 
+// ---- the usual path: one pass over the logits by independent waves, then one workgroup per row that joins them
+//
+// A wave takes a segment of a row, GROUPS loads of 16 bytes per lane, keeps it in registers and leaves the segment's
+// maximum, sum and weighted sum, and the maximum of each neighbourhood (two loads of the wave: 512 f32 or 1024 f16
+// logits that lie side by side). The best top_k logits lie in the top_k neighbourhoods with the largest maxima (ties:
+// the lower one), so the joining workgroup looks at those again and at nothing else. Bound by the one read of the logits.
+constexpr int GROUPS = 8;
+constexpr int HOODS = GROUPS / 2;          // neighbourhoods of a segment
+constexpr uint32_t MAX_HOODS = 4096;       // of a row: the joining workgroup keeps 16 per thread
+constexpr uint32_t MAX_CANDIDATES = 1024;  // logits that it ranks at once
+
+template <class T>
+constexpr uint32_t per_load = 16 / sizeof(T);
+template <class T>
+constexpr uint32_t hood_size = 2 * 64 * per_load<T>;
+template <class T>
+constexpr uint32_t segment_size = GROUPS * 64 * per_load<T>;
+
+struct SegmentStats {
+  float top, total, weighted;  // maximum of the logits; sum of e = 2^d; sum of e*d, d = (x - top) * c
+  float hood[HOODS];
+};
+
+// Elements of a row are numbered from the 16-byte boundary at or before its first one, so that every load is aligned.
+template <class T>
+__device__ __forceinline__ uint32_t lead_of(const T* row) {
+  return (uint32_t)(reinterpret_cast<uint64_t>(row) & 15u) / sizeof(T);
+}
+// per_load<T> logits from place `at` (a multiple of per_load); places outside the row read as `outside`
+template <class T>
+__device__ __forceinline__ void load_group(const T* row, uint32_t lead, uint32_t vocab, uint32_t at, float outside, float* x) {
+  constexpr uint32_t N = per_load<T>;
+  if (at >= lead && at + N <= lead + vocab) {
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+    const vec v = *reinterpret_cast<const vec*>(row + (at - lead));
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) x[i] = (float)v[i];
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) x[i] = at + i >= lead && at + i < lead + vocab ? (float)row[at + i - lead] : outside;
+  }
+}
+
+__device__ __forceinline__ float max_of_wave(float v) {
+  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  return v;
+}
+__device__ __forceinline__ float sum_of_wave(float v) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void logits_segments_kernel(const LogprobsArgs p, SegmentStats* stats, uint32_t segments, float c) {
+  constexpr uint32_t N = per_load<T>;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+  const uint32_t r = (uint32_t)(unit / segments), seg = (uint32_t)(unit - (uint64_t)r * segments);
+  if (r >= p.rows) return;  // whole waves leave together
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
+  const uint32_t lead = lead_of(row), first = seg * segment_size<T>;
+  float x[GROUPS][N];
+#pragma unroll
+  for (int g = 0; g < GROUPS; g++) load_group(row, lead, p.vocab, first + (g * 64 + lane) * N, -INFINITY, x[g]);
+  SegmentStats s;
+  s.top = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < HOODS; n++) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int g = 2 * n; g < 2 * n + 2; g++)
+#pragma unroll
+      for (uint32_t i = 0; i < N; i++) m = fmaxf(m, x[g][i]);
+    s.hood[n] = max_of_wave(m);
+    s.top = fmaxf(s.top, s.hood[n]);
+  }
+  const float top = s.top == -INFINITY ? 0.f : s.top;
+  s.total = s.weighted = 0.f;
+#pragma unroll
+  for (int g = 0; g < GROUPS; g++)
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+      const float d = (x[g][i] - top) * c, e = __builtin_amdgcn_exp2f(d);  // the difference first: exact or nearly so
+      s.total += e;
+      s.weighted = __builtin_fmaf(e, fmaxf(d, -1e4f), s.weighted);  // e is 0 there; keeps 0 * -inf out of the sum
+    }
+  s.total = sum_of_wave(s.total);
+  s.weighted = sum_of_wave(s.weighted);
+  if (lane == 0) stats[unit] = s;
+}
+
+// value and id of a candidate as one number: larger is better, ties to the lower id
+__device__ __forceinline__ unsigned long long rank_key(float v, uint32_t id) { return (unsigned long long)order_of(v) << 32 | (uint32_t)~id; }
+
+template <class T>
+__global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p, const SegmentStats* all, uint32_t segments, float c) {
+  constexpr uint32_t N = per_load<T>;
+  __shared__ float red[3][4];
+  __shared__ __align__(16) uint32_t most[256];
+  __shared__ unsigned long long candidates[MAX_CANDIDATES], best[4];
+  __shared__ uint16_t chosen[MAX_HOODS];
+  __shared__ uint32_t count, chosen_count, bound, found;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = blockIdx.x;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
+  const uint32_t lead = lead_of(row);
+  const SegmentStats* stats = all + (uint64_t)r * segments;
+  if (tid == 0) count = chosen_count = bound = found = 0;
+
+  // ---- the sums
+  float top = -INFINITY;
+  for (uint32_t s = tid; s < segments; s += 256u) top = fmaxf(top, stats[s].top);
+  top = max_of_wave(top);
+  if (lane == 0) red[0][wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const bool low = top == -INFINITY;  // nothing but -inf and NaN
+  const float m = low ? 0.f : top;
+  float total = 0.f, weighted = 0.f;
+  for (uint32_t s = tid; s < segments; s += 256u) {
+    const SegmentStats v = stats[s];
+    const float d = ((v.top == -INFINITY ? 0.f : v.top) - m) * c;  // e' = e * 2^d, (e*d)' = 2^d * (e*d + d * e)
+    const bool none = v.top == -INFINITY;
+    const float f = none ? (low ? 1.f : 0.f) : __builtin_amdgcn_exp2f(d);
+    total += v.total != v.total ? v.total : v.total * f;
+    weighted += v.total != v.total ? v.total : f == 0.f ? 0.f : f * (v.weighted + (none ? 0.f : d) * v.total);
+  }
+  total = sum_of_wave(total);
+  weighted = sum_of_wave(weighted);
+  if (lane == 0) {
+    red[1][wave] = total;
+    red[2][wave] = weighted;
+  }
+  __syncthreads();
+  total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  weighted = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  constexpr float LN2 = 0.69314718055994531f;
+  const bool nothing = low && total == 0.f;  // every logit is -inf (a NaN would be in the sum)
+  const float log_total = logf(total);
+  auto logp = [&](float v) { return nothing ? -INFINITY : ((v - m) * c) * LN2 - log_total; };
+  if (tid == 0) {
+    if (p.logprob) {
+      const int32_t t = p.tokens[r];
+      p.logprob[r] = t >= 0 && (uint32_t)t < p.vocab ? logp((float)row[t]) : -INFINITY;
+    }
+    if (p.entropy) p.entropy[r] = nothing ? 0.f : log_total - weighted / total * LN2;
+  }
+  const uint32_t K = p.top_k;
+  if (!K || (!p.top_ids && !p.top_logprobs)) return;
+  auto answer = [&](uint32_t place, unsigned long long key) {
+    const uint32_t id = ~(uint32_t)key;
+    if (p.top_ids) p.top_ids[(size_t)r * K + place] = id;
+    if (p.top_logprobs) p.top_logprobs[(size_t)r * K + place] = logp((float)row[id]);
+  };
+
+  // ---- a bound: the K-th largest of 256 maxima over disjoint parts of the row; at least K logits reach it
+  const uint32_t hoods = (lead + p.vocab + hood_size<T> - 1) / hood_size<T>;
+  const bool by_hood = hoods >= K;
+  uint32_t mine = 0;
+  if (by_hood) {
+    for (uint32_t n = tid; n < hoods; n += 256u) mine = max(mine, order_of(stats[n / HOODS].hood[n % HOODS]));
+  } else {
+    for (uint32_t i = tid; i < p.vocab; i += 256u) mine = max(mine, order_of((float)row[i]));
+  }
+  most[tid] = mine;
+  __syncthreads();
+  uint32_t above = 0;  // parts that come before this one
+#pragma unroll 1
+  for (uint32_t w = 0; w < 4; w++) {
+    const uint32_t limit = w < wave ? mine - 1u : mine;  // an equal maximum of a lower part comes first
+    if (w != wave) {
+#pragma unroll 4
+      for (uint32_t j = 64 * w; j < 64 * w + 64; j += 4) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(&most[j]);
+        above += (v.x > limit) + (v.y > limit) + (v.z > limit) + (v.w > limit);
+      }
+    } else {
+#pragma unroll 4
+      for (uint32_t j = 0; j < 64; j++) {
+        const uint32_t v = most[64 * w + j];
+        above += v > mine || (v == mine && j < lane);
+      }
+    }
+  }
+  if (mine && above == K - 1) bound = mine;
+  __syncthreads();
+  const uint32_t least = bound;
+
+  // ---- the neighbourhoods that reach the bound, and every logit of theirs that does
+  if (by_hood) {
+    for (uint32_t n = tid; n < hoods; n += 256u)
+      if (order_of(stats[n / HOODS].hood[n % HOODS]) >= least) chosen[atomicAdd(&chosen_count, 1u)] = (uint16_t)n;
+    __syncthreads();
+  }
+  // f(value, id) for every logit that can be among the best
+  auto each = [&](auto&& f) {
+    if (by_hood) {
+      for (uint32_t k = wave; k < chosen_count; k += 4u) {
+        const uint32_t first = (uint32_t)chosen[k] * hood_size<T>;
+#pragma unroll
+        for (uint32_t g = 0; g < 2; g++) {
+          float x[N];
+          const uint32_t at = first + (g * 64 + lane) * N;
+          load_group(row, lead, p.vocab, at, 0.f, x);
+#pragma unroll
+          for (uint32_t i = 0; i < N; i++)
+            if (at + i >= lead && at + i < lead + p.vocab) f(x[i], at + i - lead);
+        }
+      }
+    } else {
+      for (uint32_t i = tid; i < p.vocab; i += 256u) f((float)row[i], i);
+    }
+  };
+  auto collect = [&](uint32_t from) {  // logits whose order is at least `from`
+    each([&](float v, uint32_t id) {
+      if (order_of(v) >= from) {
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < MAX_CANDIDATES) candidates[at] = rank_key(v, id);
+      }
+    });
+    __syncthreads();
+  };
+  auto rank = [&](uint32_t n) {  // places of the first n candidates
+    for (uint32_t i = tid; i < n; i += 256u) {
+      const unsigned long long key = candidates[i];
+      uint32_t place = 0;
+      for (uint32_t j = 0; j < n; j++) place += candidates[j] > key;
+      if (place < K) answer(place, key);
+    }
+  };
+  collect(least);
+  const uint32_t reached = count;
+  if (reached >= K && reached <= MAX_CANDIDATES) {
+    rank(reached);
+    return;
+  }
+  // ---- many equal logits (a row that is masked but for a few): those above the bound, then the bound's own value in
+  // the order of the ids
+  __syncthreads();
+  if (tid == 0) count = 0;
+  __syncthreads();
+  if (reached > MAX_CANDIDATES) {
+    collect(least + 1);
+    const uint32_t over = count;
+    if (over < K) {
+      rank(over);
+      uint32_t have = over;
+      for (uint32_t i0 = 0; i0 < p.vocab && have < K; i0 += 256u) {
+        const uint32_t i = i0 + tid;
+        const bool hit = i < p.vocab && order_of((float)row[i]) == least;
+        const unsigned long long ballot = __ballot(hit);
+        if (lane == 0) most[wave] = (uint32_t)__popcll(ballot);
+        __syncthreads();
+        uint32_t place = have + (uint32_t)__popcll(ballot & ((1ull << lane) - 1ull));
+        for (uint32_t w = 0; w < wave; w++) place += most[w];
+        if (hit && place < K) answer(place, rank_key((float)row[i], i));
+        have += most[0] + most[1] + most[2] + most[3];
+        __syncthreads();
+      }
+      return;
+    }
+    if (over <= MAX_CANDIDATES) {
+      rank(over);
+      return;
+    }
+  }
+  // ---- anything else (rows in order, rows of NaN): one alternative after the other
+  unsigned long long last = ~0ull;
+  for (uint32_t k = 0; k < K; k++) {
+    unsigned long long key = 0;
+    auto look = [&](float v, uint32_t id) {
+      const unsigned long long x = rank_key(v, id);
+      if (x < last && x > key) key = x;
+    };
+    if (reached >= K) each(look);
+    else
+      for (uint32_t i = tid; i < p.vocab; i += 256u) look((float)row[i], i);
+    for (int o = 32; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor(key, o);
+      key = other > key ? other : key;
+    }
+    if (lane == 0) best[wave] = key;
+    __syncthreads();
+    last = best[0];
+    for (uint32_t w = 1; w < 4; w++) last = best[w] > last ? best[w] : last;
+    __syncthreads();
+    if (tid == 0) answer(k, last);
+  }
+}
+
+// Segments of a row, whatever its alignment.
+template <class T>
+uint32_t segments_of(uint32_t vocab) {
+  return (uint32_t)(((uint64_t)vocab + per_load<T> - 1 + segment_size<T> - 1) / segment_size<T>);
+}
+template <class T>
+bool segmented(uint32_t vocab) {
+  return (uint64_t)vocab + per_load<T> <= (uint64_t)MAX_HOODS * hood_size<T>;
+}
+template <class T>
+hipError_t launch_typed(const LogprobsArgs& a, void* scratch, hipStream_t s) {
+  if (!segmented<T>(a.vocab)) {
+    hipLaunchKernelGGL(logprobs_any_kernel<T>, dim3(a.rows), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  SegmentStats* stats = static_cast<SegmentStats*>(scratch);
+  const uint32_t segments = segments_of<T>(a.vocab);
+  const float c = a.inv_temperature * 1.4426950408889634f;
+  const uint64_t waves = (uint64_t)a.rows * segments;
+  hipLaunchKernelGGL(logits_segments_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, a, stats, segments, c);
+  hipLaunchKernelGGL(logits_answer_kernel<T>, dim3(a.rows), dim3(256), 0, s, a, stats, segments, c);
+  return hipGetLastError();
+}
+
 }  // namespace
 
-hipError_t launch_logprobs(const LogprobsArgs& a, hipStream_t s) {
-  if (a.f16) hipLaunchKernelGGL(logprobs_kernel<_Float16>, dim3(a.rows), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(logprobs_kernel<float>, dim3(a.rows), dim3(256), 0, s, a);
-  return hipGetLastError();
+size_t logprobs_scratch_bytes(const LogprobsArgs& a) {
+  const bool takes = a.f16 ? segmented<_Float16>(a.vocab) : segmented<float>(a.vocab);
+  return takes ? (size_t)a.rows * (a.f16 ? segments_of<_Float16>(a.vocab) : segments_of<float>(a.vocab)) * sizeof(SegmentStats) : 0;
+}
+
+hipError_t launch_logprobs(const LogprobsArgs& a, void* scratch, hipStream_t s) {
+  return a.f16 ? launch_typed<_Float16>(a, scratch, s) : launch_typed<float>(a, scratch, s);
 }
 
 }  // namespace ztvm

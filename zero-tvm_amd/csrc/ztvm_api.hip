@@ -975,7 +975,7 @@ int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* d) {
   if (d->row_stride < d->vocab) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: row_stride=%u is less than vocab=%u", d->row_stride, d->vocab);
   if (d->logits_f16 > 1) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: logits_f16 must be 0 or 1");
   if (d->top_k > 64u || d->top_k > d->vocab) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: top_k must be 0..min(vocab, 64) (got %u of %u)", d->top_k, d->vocab);
-  if (!(d->inv_temperature > 0.f) || !std::isfinite(d->inv_temperature)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: inv_temperature must be > 0 and finite");
+  if (!(d->inv_temperature > 0.f) || !(d->inv_temperature <= 1e38f)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: inv_temperature must be > 0 and at most 1e38");
   if (!d->logits) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: null logits");
   if (d->logprob && !d->tokens) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: logprob needs tokens");
   if ((d->logits & (d->logits_f16 ? 1u : 3u)) || ((d->tokens | d->logprob | d->entropy | d->top_ids | d->top_logprobs) & 3u))
@@ -994,7 +994,13 @@ int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* d) {
   a.inv_temperature = d->inv_temperature;
   DeviceGuard g(ctx->device);
   if (!g.ok) return fail(ctx, ZTVM_E_HIP, "ztvm_token_logprobs: hipSetDevice(%d) failed", ctx->device);
-  HIP_TRY(ctx, launch_logprobs(a, ctx->stream));
+  void* scratch = nullptr;
+  const size_t need = logprobs_scratch_bytes(a);
+  if (need) {
+    const int rc = scratch_for(ctx, need, &scratch);
+    if (rc) return rc;
+  }
+  HIP_TRY(ctx, launch_logprobs(a, scratch, ctx->stream));
   return ZTVM_OK;
 }
 
