@@ -155,6 +155,7 @@ __device__ __forceinline__ constexpr uint32_t swz_v(uint32_t row) {  // pairs of
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(4))) int32_t* const_i32;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 struct MfmaParams {
@@ -218,7 +219,7 @@ struct MfmaShape {
   static constexpr int ROWS = 16 * QT * RW;
   static constexpr int STAGES = RW == 1 ? 2 : 3;
   static constexpr int PART = 32 * DIM * (INT8 ? 2 : 4);  // bytes of 32 keys: K then V (int8: rows of K | V)
-  static constexpr int SCALES = INT8 ? 32 * 4 : 0;
+  static constexpr int SCALES = INT8 ? 256 : 0;
   static constexpr int STAGE = KW * (PART + SCALES);
   static constexpr int PITCH = DIM + 4;  // of the joined rows
   static constexpr int JOIN = KW > 1 ? KW * ROWS * PITCH * 4 + KW * ROWS * 8 : 0;
@@ -226,12 +227,13 @@ struct MfmaShape {
 };
 
 template <int KD, bool INT8, int QT, int RW, int KW>
-__global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const MfmaParams p) {
+__global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_kernel(const MfmaParams p) {
   using Shape = MfmaShape<KD, INT8, QT, RW, KW>;
   constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, ST = Shape::STAGES;
   constexpr float THR = INT8 ? 2.f : 6.f, LIFT = INT8 ? 16.f : 512.f;  // probabilities stay below 2^THR * LIFT (* 515, int8): f16's range
   constexpr int MOVES = INT8 ? KD * 2 : KD * 4;     // transfers of 1 KiB that bring 32 keys
-  constexpr int DMA = (MOVES + RW - 1) / RW;        // of which a wave makes so many (the last one twice where they do not share evenly)
+  constexpr int MOVES_EACH = (MOVES + RW - 1) / RW;  // of which a wave makes so many (the last one twice where they do not share evenly)
+  constexpr int DMA = MOVES_EACH + (INT8 ? 1 : 0);   // and the scales
   extern __shared__ __align__(16) char lds[];
   const AttentionArgs& a = p.a;
   const KvView& c = a.cache;
@@ -288,58 +290,57 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   // KD transfers move 16 rows of one side (f16) or of both (int8, K | V). Transfer g of the MOVES that bring 32 keys:
   // f16: K of keys 0-15, of 16-31, then V; int8: keys 0-15, 16-31. A wave makes those of its turn among the RW.
-  uint32_t voff[DMA];
+  uint32_t voff[MOVES_EACH];
 #pragma unroll
-  for (int i = 0; i < DMA; i++) {
+  for (int i = 0; i < MOVES_EACH; i++) {
     const uint32_t g = min((uint32_t)i * RW + rw, MOVES - 1u), within = g % (2 * KD);
     const uint32_t idx = within * 64 + lane, row = idx / (4 * KD), ch = idx - row * (4 * KD);
     const uint32_t swz = INT8 || g < 2 * KD ? swz_k<KD>(row) : swz_v<KD>(row);
     voff[i] = (row & 15u) * c.slot_bytes + ((ch ^ swz) * 16);
   }
   const char* head_base = c.pages + (uint64_t)h * c.head_bytes;
-  auto base_of = [&](int32_t pos, bool& valid) -> const char* {  // 16 keys from pos on; uniform
-    uint32_t page = 0, slot = 0;
-    valid = pos < k_end;
-    if (valid) {
-      const uint32_t pno = fast_div(c.by_page, (uint32_t)pos);
-      slot = (uint32_t)pos - pno * c.page_size;
-      page = a.page_table ? (uint32_t)a.page_table[(size_t)b * a.page_table_stride + pno] : pno;
-      valid = page < c.num_pages;
-    }
-    if (!valid) page = slot = 0;  // some rows that exist; nobody sees them
-    return head_base + (uint64_t)page * c.page_bytes + (uint64_t)slot * c.slot_bytes;
+  // Page numbers come through the scalar cache (the constant address space makes the compiler load them so): a vector
+  // load here would have to wait for every transfer in flight.
+  const const_i32 table = (const_i32)(uintptr_t)(a.page_table ? a.page_table + (size_t)b * a.page_table_stride : nullptr);
+  struct Block {  // 16 keys
+    uint32_t page, slot;
+    bool inside;
   };
-  auto scales_of = [&](int32_t pos) -> const char* {
-    uint32_t page = 0, slot = 0;
-    if (pos < k_end) {
-      const uint32_t pno = fast_div(c.by_page, (uint32_t)pos);
-      slot = (uint32_t)pos - pno * c.page_size;
-      page = a.page_table ? (uint32_t)a.page_table[(size_t)b * a.page_table_stride + pno] : pno;
-      if (page >= c.num_pages) page = slot = 0;
-    }
-    return reinterpret_cast<const char*>(c.scales + kv_scale_index(c, page, h, slot, 0));
+  auto block_at = [&](int32_t pos) {
+    Block x;
+    const uint32_t at = (uint32_t)min(pos, k_end - 1);  // always a position there is
+    const uint32_t pno = fast_div(c.by_page, at);
+    x.slot = (at - pno * c.page_size) & ~15u;
+    x.page = table ? (uint32_t)table[pno] : pno;
+    x.inside = pos < k_end;
+    return x;
   };
-  auto issue = [&](int32_t turn, uint32_t stage) {
-    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
+  auto settle_block = [&](Block& x) {  // some rows that exist where the page is none; nobody sees them
+    x.inside = x.inside && x.page < c.num_pages;
+    if (!x.inside) x.page = x.slot = 0;
+  };
+  auto base_of = [&](const Block& x) { return head_base + (uint64_t)x.page * c.page_bytes + (uint64_t)x.slot * c.slot_bytes; };
+  auto key_of = [&](int32_t turn) { return k_begin + 32 * (int32_t)(kw + KW * turn); };
+  // starts the transfers of a turn's 32 keys; returns which halves are inside the cache
+  auto issue = [&](Block x0, Block x1, uint32_t stage) -> uint32_t {
+    settle_block(x0);
+    settle_block(x1);
     const uint32_t at = lds_base + stage * Shape::STAGE + kw * Shape::PART;
-    bool ok0, ok1;
-    const char* base0 = base_of(pos, ok0);
-    const char* base1 = base_of(pos + 16, ok1);
-    static_for<DMA>([&](auto i_) {
+    const char* base0 = base_of(x0);
+    const char* base1 = base_of(x1);
+    static_for<MOVES_EACH>([&](auto i_) {
       constexpr int i = decltype(i_)::value;
       const uint32_t g = min((uint32_t)i * RW + rw, MOVES - 1u);
       const char* base = g / KD % 2 ? base1 : base0;
       if (!INT8 && g >= 2 * KD) base += c.side_bytes;
       dma16<0>(base, voff[i], at + 1024u * g);
     });
-  };
-  // int8 scales of the wave's 32 keys, K | V per key: lane j < 32 holds key j's pair
-  auto fetch_scales = [&](int32_t turn) -> uint32_t {
-    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
-    const char* s0 = scales_of(pos);
-    const char* s1 = scales_of(pos + 16);
-    const char* s = lane & 16u ? s1 : s0;
-    return *reinterpret_cast<const uint32_t*>(s + 4u * lj);
+    if constexpr (INT8) {  // a pair of scales for each key (lanes 32..63 repeat them)
+      const uint32_t key = lane & 31u;
+      const uint64_t s0 = kv_scale_index(c, x0.page, h, x0.slot, 0), s1 = kv_scale_index(c, x1.page, h, x1.slot, 0);
+      dma4(reinterpret_cast<const char*>(c.scales + (key < 16 ? s0 : s1)) + 4u * (key & 15u), lds_base + stage * Shape::STAGE + KW * Shape::PART + kw * Shape::SCALES);
+    }
+    return (x0.inside ? 1u : 0u) | (x1.inside ? 2u : 0u);
   };
 
   f4 acc[QT][2 * KD];
@@ -352,8 +353,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
     for (int d = 0; d < 2 * KD; d++) acc[t][d] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto compute = [&](int32_t turn, uint32_t stage, uint32_t scale_pair) {
-    const int32_t pos = k_begin + 32 * (int32_t)(kw + KW * turn);
+  auto compute = [&](int32_t turn, uint32_t stage, uint32_t inside) {
+    const int32_t pos = key_of(turn);
     if (pos >= k_end) return;
     const char* kv = lds + stage * Shape::STAGE + kw * Shape::PART;
     f4 s[QT][2];
@@ -378,22 +379,19 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
     // scales: log2 units of the scores, and what the values' rows weigh
     float ks[2][4], vs[2][4];
     if constexpr (INT8) {
+      const char* pairs = lds + stage * Shape::STAGE + KW * Shape::PART + kw * Shape::SCALES;
 #pragma unroll
-      for (int half = 0; half < 2; half++)
+      for (int half = 0; half < 2; half++) {
+        const u32x4 four = *reinterpret_cast<const u32x4*>(pairs + 64 * half + 16 * lc);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const h2 pair = as_h2(__builtin_amdgcn_ds_bpermute((int)(4u * (16 * half + 4 * lc + i)), (int)scale_pair));
+          const h2 pair = as_h2(four[i]);
           ks[half][i] = (float)pair.x * p.scale_log2;
           vs[half][i] = (float)pair.y * LIFT;
         }
+      }
     }
-    bool edge = pos + 32 > full;
-    bool ok0 = true, ok1 = true;
-    if (!edge) {
-      base_of(pos, ok0);
-      base_of(pos + 16, ok1);
-      edge = !(ok0 && ok1);
-    }
+    const bool edge = pos + 32 > full || inside != 3u;
     h8 pf[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -404,9 +402,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
         for (int i = 0; i < 4; i++) x[half][i] = s[t][half][i] * (INT8 ? ks[half][i] : p.scale_log2);
       uint32_t seen = ~0u;
       if (edge) {
-        base_of(pos, ok0);
-        base_of(pos + 16, ok1);
-        seen = visible_bits(pos, context, limit[t], words[t], a.mask_words) & (ok0 ? ~0u : 0xFFFF0000u) & (ok1 ? ~0u : 0x0000FFFFu);
+        seen = visible_bits(pos, context, limit[t], words[t], a.mask_words) & (inside & 1u ? ~0u : 0xFFFF0000u) & (inside & 2u ? ~0u : 0x0000FFFFu);
         seen >>= 4 * lc;
 #pragma unroll
         for (int half = 0; half < 2; half++)
@@ -489,32 +485,33 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
   };
 
   // ---- the pipeline
-  if constexpr (RW == 1) {  // a wave's keys are its own: no barrier
+  uint32_t halves = 0;  // two bits for each stage in flight, the oldest lowest
+  if constexpr (RW == 1) {  // a wave's keys are its own: no barrier; a stage is filled again as soon as it has been used
 #pragma unroll
     for (int i = 0; i < ST; i++)
-      if (i < turns) issue(i, i);
+      if (i < turns) halves |= issue(block_at(key_of(i)), block_at(key_of(i) + 16), i) << (2 * i);
     for (int32_t turn = 0; turn < turns; turn++) {
       const uint32_t stage = turn % ST;
-      uint32_t pair_now = 0;
-      if constexpr (INT8) pair_now = fetch_scales(turn);
-      if (turn + 1 < turns) wait_vm<(ST - 1) * DMA>();
+      const Block x0 = block_at(key_of(turn + ST)), x1 = block_at(key_of(turn + ST) + 16);
+      if (turn + ST - 1 < turns) wait_vm<(ST - 1) * DMA>();
       else wait_vm<0>();
-      compute(turn, stage, pair_now);
+      compute(turn, stage, halves & 3u);
+      halves >>= 2;
       wait_lgkm<0>();
-      if (turn + ST < turns) issue(turn + ST, stage);
+      if (turn + ST < turns) halves |= issue(x0, x1, stage) << (2 * (ST - 1));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < ST - 1; i++)
-      if (i < turns) issue(i, i);
+      if (i < turns) halves |= issue(block_at(key_of(i)), block_at(key_of(i) + 16), i) << (2 * i);
     for (int32_t turn = 0; turn < turns; turn++) {
-      uint32_t pair_now = 0;
-      if constexpr (INT8) pair_now = fetch_scales(turn);
-      if (turn + 1 < turns) wait_vm<(ST - 2) * DMA>();
+      const Block x0 = block_at(key_of(turn + ST - 1)), x1 = block_at(key_of(turn + ST - 1) + 16);
+      if (turn + ST - 2 < turns) wait_vm<(ST - 2) * DMA>();
       else wait_vm<0>();
       wg_barrier();  // everybody's transfers of this stage have landed, everybody has left the stage before
-      if (turn + ST - 1 < turns) issue(turn + ST - 1, (turn + ST - 1) % ST);
-      compute(turn, turn % ST, pair_now);
+      if (turn + ST - 1 < turns) halves |= issue(x0, x1, (turn + ST - 1) % ST) << (2 * (ST - 1));
+      compute(turn, turn % ST, halves & 3u);
+      halves >>= 2;
       wait_lgkm<0>();
     }
   }
@@ -593,7 +590,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mfma_kernel(const Mfma
 }
 
 // Adds the partial results of a row's splits, in their order. One wave per query row and head.
-__global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t rows_per_wg, uint32_t causal_rows, float lift) {
+__global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t tile_rows, float lift) {
   const AttentionArgs& a = p.a;
   const KvView& c = a.cache;
   const uint32_t lane = threadIdx.x & 63u, b = blockIdx.y;
@@ -606,26 +603,38 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
   const int32_t length = min(max(a.kv_length[b], 0), (int32_t)a.max_kv);
   const int64_t context = length - n;
   // how many splits the row's workgroup had, as it worked it out
-  const uint32_t last_row = min(row / causal_rows * causal_rows + causal_rows, (uint32_t)tokens * p.group) - 1;
+  const uint32_t last_row = min(row / tile_rows * tile_rows + tile_rows, (uint32_t)tokens * p.group) - 1;
   const int64_t seen_by_any = a.tree_mask ? length : context + last_row / p.group + 1;
   const int32_t k_last = (int32_t)max(min(seen_by_any, (int64_t)length), (int64_t)0);
   const uint32_t parts = max(1u, ((uint32_t)k_last + p.chunk - 1) / p.chunk);
   if (parts == 1) return;
   const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits;
+  const float* acc = p.partial + at * c.head_dim;
+  const float2* ml = p.partial_ml + at;
   float top = NOTHING;
-  for (uint32_t s = lane; s < parts; s += 64u) top = fmaxf(top, p.partial_ml[at + s].x);
+  for (uint32_t s = lane; s < parts; s += 64u) top = fmaxf(top, ml[s].x);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  float total = 0.f;
-  for (uint32_t s = lane; s < parts; s += 64u) total += p.partial_ml[at + s].y * __builtin_amdgcn_exp2f(p.partial_ml[at + s].x - top);
+  float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};  // dims lane, lane + 64, ..
+  for (uint32_t s0 = 0; s0 < parts; s0 += 64u) {
+    const uint32_t here = min(parts - s0, 64u);
+    const float2 mine = lane < here ? ml[s0 + lane] : make_float2(NOTHING, 0.f);
+    const float w = lane < here ? __builtin_amdgcn_exp2f(mine.x - top) : 0.f;
+    total += mine.y * w;
+#pragma unroll 8
+    for (uint32_t s = 0; s < here; s++) {
+      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (int)s));
+#pragma unroll
+      for (uint32_t k = 0; k < 4; k++)
+        if (lane + 64u * k < c.head_dim) v[k] += acc[(size_t)(s0 + s) * c.head_dim + lane + 64u * k] * ws;
+    }
+  }
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
   const float inv = total > 0.f || total != total ? 1.0f / (total * lift) : 0.f;
   const uint32_t i = row / p.group, head = h * p.group + (row - i * p.group);
   _Float16* out = a.out + (size_t)(start + i) * a.out_stride + (size_t)head * c.head_dim;
-  for (uint32_t d = lane; d < c.head_dim; d += 64u) {
-    float v = 0.f;
-    for (uint32_t s = 0; s < parts; s++) v += p.partial[(at + s) * c.head_dim + d] * __builtin_amdgcn_exp2f(p.partial_ml[at + s].x - top);
-    out[d] = narrow_f32(v * inv);
-  }
+#pragma unroll
+  for (uint32_t k = 0; k < 4; k++)
+    if (lane + 64u * k < c.head_dim) out[lane + 64u * k] = narrow_f32(v[k] * inv);
   if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top + __log2f(total)) * 0.69314718055994531f : -INFINITY;
 }
 
@@ -648,19 +657,25 @@ struct MfmaPlan {
   uint32_t rows, row_tiles, splits, chunk;
   size_t partial_bytes, bytes;
 };
+#ifndef ATTN_KW1
+#define ATTN_KW1 2
+#endif
 MfmaPlan mfma_plan(const AttentionArgs& a) {
   MfmaPlan g{};
   const uint32_t group = a.heads / a.cache.kv_heads;
   const uint64_t rows = (uint64_t)std::min(a.max_query, a.tokens) * group;
   const bool wide = a.cache.head_dim > 128;
-  if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = wide ? 2 : 4;
+  if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = wide ? 2 : ATTN_KW1;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
   else g.qt = 2, g.rw = 4, g.kw = 1;
   g.rows = 16 * g.qt * g.rw;
   g.row_tiles = (uint32_t)((rows + g.rows - 1) / g.rows);
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
   // enough workgroups for a few rounds of the CUs, none with less than four turns of its waves
-  const uint64_t want = 1024;
+#ifndef ATTN_WANT
+#define ATTN_WANT 1024
+#endif
+  const uint64_t want = ATTN_WANT;
   const uint32_t least = 32u * g.kw * 4u;
   uint64_t splits = (want + groups - 1) / groups;
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (a.max_kv + least - 1) / least));
@@ -684,7 +699,7 @@ hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.splits == 1) return e;
   const uint32_t units = std::min(p.a.max_query, p.a.tokens) * p.a.heads;
-  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, 0u, (uint32_t)g.rows, INT8 ? 16.f : 512.f);
+  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, INT8 ? 16.f : 512.f);
   return hipGetLastError();
 }
 template <int KD, bool INT8>
@@ -692,7 +707,7 @@ hipError_t launch_mfma_dim(const MfmaParams& p, const MfmaPlan& g, hipStream_t s
   constexpr int KW = KD > 4 ? 2 : 4;
   if (g.rw == 4) return launch_mfma_shape<KD, INT8, 2, 4, 1>(p, g, s);
   if (g.qt == 2) return launch_mfma_shape<KD, INT8, 2, 1, KW>(p, g, s);
-  return launch_mfma_shape<KD, INT8, 1, 1, KW>(p, g, s);
+  return launch_mfma_shape<KD, INT8, 1, 1, (KD > 4 ? 2 : ATTN_KW1)>(p, g, s);
 }
 
 }  // namespace

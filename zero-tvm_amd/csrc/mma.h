@@ -43,6 +43,10 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t 
                : "v"(voff), "s"(base), "s"(lds_base - OFF), "n"(OFF)
                : "memory", "m0");
 }
+// 4 bytes per lane: global (the lane's address) -> LDS (lds_base + 4*lane)
+__device__ __forceinline__ void dma4(const void* addr, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(addr), "s"(lds_base) : "memory", "m0");
+}
 template <int OFF>
 __device__ __forceinline__ void fetch32(uint32_t& v, const void* base, uint32_t voff) {
   asm volatile("global_load_dword %0, %1, %2 offset:%3" : "=v"(v) : "v"(voff), "s"(base), "n"(OFF));
