@@ -173,6 +173,30 @@ def test_infinities_in_masked_places(ctx, capi, dim, heads):
             assert not np.all(np.isfinite(out[2].astype(np.float64)))
 
 
+@pytest.mark.parametrize("dim,heads,queries", [(128, 4, 6), (96, 14, 6), (64, 16, 6), (128, 2, 40), (20, 2, 6)])
+def test_scales_that_are_no_numbers_in_masked_places(ctx, capi, dim, heads, queries):
+    for bad in (np.inf, np.nan, -np.inf):
+        s = Step(23, heads, 2, dim, 16, [(queries, 70), (3, 3), (1, 33)], True, tree="tree")
+        q, sc = s.cache
+        used = np.zeros((sc.shape[0], 16), bool)
+        for b, n in enumerate(s.lengths):
+            for p in range(n):
+                used[s.table[b, p // 16], p % 16] = True
+        sc.transpose(0, 2, 1, 3)[~used] = bad
+        s.check(ctx, capi)
+        s = Step(24, heads, 2, dim, 16, [(6, 37)], True, tree=[0b1, 0b11, 0b101, 0b1001, 0b10001, 0b100001])
+        want = s.want()
+        page, slot = s.table[0, 33 // 16], 33 % 16                          # token 2 of the tree
+        s.cache[1][page, :, slot] = bad
+        with Dev(ctx) as d:
+            ctx.attention(s.desc(ctx, capi, d))
+            out, lse = s.got(ctx)
+        keep = [0, 1, 3, 4, 5]
+        ref.close_attention(out[keep].reshape(5, heads, dim), lse[keep], *(w[keep] for w in want), dim, 37)
+        if np.isnan(bad):                                                   # an infinite score may be one of probability zero
+            assert not np.all(np.isfinite(out[2].astype(np.float64)))
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("dim", [128, 64, 20])
 def test_bad_pages_and_lengths(ctx, capi, int8, dim):

@@ -5,6 +5,7 @@
 #include "quant.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ztvm {
 namespace {
@@ -135,7 +136,9 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
 //
 // The running maximum is lazy: a row's reference value moves only when a score exceeds it by 2^THR, so most tiles need no
 // exchange between lanes and no rescaling. Probabilities are lifted by 2^LIFT before they round to f16, which keeps
-// small ones out of its subnormal range; int8 keys' scales multiply the scores, int8 values' scales the probabilities.
+// small ones out of its subnormal range; int8 keys' scales multiply the scores, int8 values' scales the probabilities
+// (their power of two goes into the widened values where those are made once for several waves: exact, and the
+// probabilities keep their range).
 //
 // Keys and values travel global -> LDS without passing registers, 32 keys a wave and stage, 16-byte chunks XOR-swizzled
 // so that neither kind of read meets bank conflicts. A page holds a multiple of 16 slots here, so 16 keys always lie in
@@ -145,12 +148,15 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
 // the row bits that the pitch does not.
 template <int KD>
 __device__ __forceinline__ constexpr uint32_t swz_k(uint32_t row) {
-  const uint32_t hi = row >> 4;  // tells rows 16 apart: the 8-bit transposing read takes rows r and r + 16 together
-  return KD % 4 == 0 ? (row & 15u) ^ (hi << 3) : KD % 2 == 0 ? ((row >> 1) & 7u) ^ (hi << 2) : ((row >> 2) & 3u) ^ (hi << 1);
+  return KD % 4 == 0 ? row & 15u : KD % 2 == 0 ? (row >> 1) & 7u : (row >> 2) & 3u;
 }
 template <int KD>
 __device__ __forceinline__ constexpr uint32_t swz_v(uint32_t row) {  // pairs of chunks over eight rows
   return KD % 4 == 0 ? (row & 7u) << 1 : KD % 2 == 0 ? ((row >> 1) & 3u) << 1 : ((row >> 2) & 1u) << 1;
+}
+template <int KD>
+__device__ __forceinline__ constexpr uint32_t swz_i8(uint32_t row) {  // the 8-bit transposing read takes rows r and r + 16 together
+  return swz_k<KD>(row) ^ ((row >> 4) << (KD % 4 == 0 ? 3 : KD % 2 == 0 ? 2 : 1));
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -161,12 +167,15 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 struct MfmaParams {
   AttentionArgs a;
   float* partial;   // [sequence][head][row of max_query tokens][split][dim], times 2^LIFT
-  float2* partial_ml;  // reference value (log2) and sum
+  float2* partial_ml;  // reference value (log2) and sum, times 2^LIFT
+  uint32_t* arrivals;  // of the workgroups that split a row tile, one counter each; zero between launches
   uint32_t splits, chunk, group;
   float scale_log2;  // |scale| * log2 e
   uint32_t negate;   // scale < 0: the queries change sign
 };
 
+constexpr float lift_of(bool raw_int8) { return raw_int8 ? 4.f : 9.f; }
+constexpr int MOST_SPLITS = 128;
 constexpr float NOTHING = -3.0e38f;  // a row's reference value before its first key
 
 __device__ __forceinline__ float across_groups_max(float v) {
@@ -189,48 +198,77 @@ __device__ __forceinline__ h8 widen_i8(u32x2 w) {
   return h8{r0.x, r0.y, r1.x, r1.y, r2.x, r2.y, r3.x, r3.y};
 }
 
-// Which keys k0 .. k0+31 a query token sees: bit j. `limit`: the first position it cannot see in any case.
-__device__ __forceinline__ uint32_t visible_bits(int64_t k0, int64_t context, int64_t limit, const uint64_t* words, uint32_t mask_words) {
+// 2^s nearest to an f16 scale from below, with s in -13..9 so that 127 * 2^s and 2^s are f16 numbers; 1 for what is no number
+__device__ __forceinline__ _Float16 power_of(uint16_t scale) {
+  uint32_t e = scale >> 10 & 31u;
+  e = e == 31u ? 15u : min(max(e, 2u), 24u);
+  return __builtin_bit_cast(_Float16, (uint16_t)(e << 10));
+}
+
+// Which of the keys k0 .. k0+63 a query token sees: bit j. `limit`: the first position it cannot see in any case; words: its
+// mask, null without a tree.
+__device__ __forceinline__ uint64_t visible_bits(int64_t k0, int64_t context, int64_t limit, const uint64_t* words, uint32_t mask_words) {
   const int64_t left = limit - k0;
-  uint32_t bits = left <= 0 ? 0u : left >= 32 ? ~0u : (1u << left) - 1u;
+  uint64_t bits = left <= 0 ? 0ull : left >= 64 ? ~0ull : (1ull << left) - 1ull;
   if (words && bits) {
     const int64_t rel = k0 - context;  // bit of the first key; below zero: history
-    uint32_t seen;
-    if (rel <= -32) {
-      seen = ~0u;
-    } else if (rel < 0) {
-      const uint32_t n = (uint32_t)-rel;
-      seen = (uint32_t)(words[0] << n) | ((1u << n) - 1u);
+    if (rel < 0) {
+      if (rel > -64) bits &= words[0] << -rel | ((1ull << -rel) - 1ull);
     } else {
       const uint64_t w = (uint64_t)rel >> 6;
       const uint32_t b = (uint32_t)rel & 63u;
-      uint64_t v = w < mask_words ? words[w] >> b : 0ull;
-      if (b > 32u && w + 1 < mask_words) v |= words[w + 1] << (64u - b);
-      seen = (uint32_t)v;
+      uint64_t v = (w < mask_words ? words[w] : 0ull) >> b;
+      if (b && w + 1 < mask_words) v |= words[w + 1] << (64u - b);
+      bits &= v;
     }
-    bits &= seen;
   }
   return bits;
 }
 
-template <int KD, bool INT8, int QT, int RW, int KW>
+// an address that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
+}
+
+// NS: 32-key tiles that a wave takes a turn
+template <int KD, bool INT8, int QT, int RW, int KW, int NS>
 struct MfmaShape {
   static constexpr int DIM = 32 * KD;
   static constexpr int ROWS = 16 * QT * RW;
   static constexpr int STAGES = RW == 1 ? 2 : 3;
-  static constexpr int PART = 32 * DIM * (INT8 ? 2 : 4);  // bytes of 32 keys: K then V (int8: rows of K | V)
+  static constexpr int KEYS = 32 * NS;
+  static constexpr int PART = 32 * DIM * (INT8 ? 2 : 4);  // bytes of 32 keys as they arrive: K then V (int8: rows of K | V)
   static constexpr int SCALES = INT8 ? 256 : 0;
   static constexpr int STAGE = KW * (PART + SCALES);
-  static constexpr int PITCH = DIM + 4;  // of the joined rows
-  static constexpr int JOIN = KW > 1 ? KW * ROWS * PITCH * 4 + KW * ROWS * 8 : 0;
-  static constexpr int LDS = std::max(STAGES * STAGE, JOIN);
+  static constexpr bool WIDEN = INT8 && RW > 1;            // int8 rows become f16 once for all waves
+  static constexpr int PAIRS = KEYS * DIM * 4;             // in a widened tile: K, V, then the scales of each as f32,
+  static constexpr int FLAGS = PAIRS + KEYS * 8;           // then which of its 16-key blocks are inside the cache
+  static constexpr int WIDE = WIDEN ? FLAGS + 16 : 0;
+  static_assert(WIDEN || NS == 1, "only the widened tiles are made of several");
+  static_assert(!WIDEN || (RW == 4 && NS == 2), "a wave widens one 16-key block");
+  static constexpr int PITCH = DIM + 4;                    // of the joined rows
+  static constexpr int JOIN = KW > 1 ? std::max(KW * ROWS * PITCH * 4 + KW * ROWS * 8, ROWS * MOST_SPLITS * 8) : 0;
+  static constexpr int LDS = std::max(WIDEN ? 2 * WIDE : STAGES * STAGE, JOIN);
 };
 
-template <int KD, bool INT8, int QT, int RW, int KW>
-__global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_kernel(const MfmaParams p) {
-  using Shape = MfmaShape<KD, INT8, QT, RW, KW>;
-  constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, ST = Shape::STAGES;
-  constexpr float THR = INT8 ? 2.f : 6.f, LIFT = INT8 ? 16.f : 512.f;  // probabilities stay below 2^THR * LIFT (* 515, int8): f16's range
+// two floats past the caches that are not shared by all of the device, in one access
+__device__ __forceinline__ void put2(float* to, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, make_float2(x, y)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* from) {
+  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+template <int KD, bool INT8, int QT, int RW, int KW, int NS>
+__global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS == 1 ? 4 : 2) void attention_mfma_kernel(const MfmaParams p) {
+  using Shape = MfmaShape<KD, INT8, QT, RW, KW, NS>;
+  constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, ST = Shape::STAGES, KEYS = Shape::KEYS;
+  // probabilities enter f16 times 2^LIFT and stay below 2^(THR + LIFT): inside f16's range. Where int8 scales multiply them
+  // as they are, times 515 more (the largest scale whose 127 counts f16 can hold).
+  constexpr bool RAW8 = INT8 && !Shape::WIDEN;
+  constexpr float LIFT = lift_of(RAW8), CAP = RAW8 ? 64.f : 32768.f;  // CAP = 2^(THR + LIFT)
   constexpr int MOVES = INT8 ? KD * 2 : KD * 4;     // transfers of 1 KiB that bring 32 keys
   constexpr int MOVES_EACH = (MOVES + RW - 1) / RW;  // of which a wave makes so many (the last one twice where they do not share evenly)
   constexpr int DMA = MOVES_EACH + (INT8 ? 1 : 0);   // and the scales
@@ -263,20 +301,20 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
   const uint32_t parts = max(1u, ((uint32_t)k_last + p.chunk - 1) / p.chunk);  // splits that have keys (one writes the empty rows)
   if (split >= parts) return;
   const int32_t k_begin = (int32_t)(split * p.chunk), k_end = min(k_last, k_begin + (int32_t)p.chunk);
-  const int32_t turns = (k_end - k_begin + 32 * KW - 1) / (32 * KW);
+  const int32_t turns = (k_end - k_begin + KEYS * KW - 1) / (KEYS * KW);
 
   // ---- the query rows, as B operands
   const uint32_t wave_row = row0 + rw * 16 * QT;
   h8 q[QT][KD];
-  int64_t limit[QT];          // first position the lane's row cannot see
-  const uint64_t* words[QT];  // its token's mask
+  int32_t limit[QT];   // first position the lane's row cannot see
+  uint32_t token[QT];  // whose mask it goes by
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     const uint32_t row = wave_row + 16 * t + lj, i = row / p.group;
     const bool there = row < rows;
     const _Float16* src = a.q + (size_t)(start + (there ? i : 0u)) * a.q_stride + (size_t)(h * p.group + (there ? row - i * p.group : 0u)) * DIM;
-    limit[t] = there ? (tree ? (int64_t)length : min((int64_t)length, context + i + 1)) : 0;
-    words[t] = tree ? a.tree_mask + (size_t)(start + (there ? i : 0u)) * a.mask_words : nullptr;
+    limit[t] = there ? (tree ? length : (int32_t)max(min((int64_t)length, context + i + 1), (int64_t)0)) : 0;
+    token[t] = start + (there ? i : 0u);
 #pragma unroll
     for (int s = 0; s < KD; s++) {
       u32x4 v = *reinterpret_cast<const u32x4*>(src + 32 * s + 8 * lc);
@@ -295,8 +333,8 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
   for (int i = 0; i < MOVES_EACH; i++) {
     const uint32_t g = min((uint32_t)i * RW + rw, MOVES - 1u), within = g % (2 * KD);
     const uint32_t idx = within * 64 + lane, row = idx / (4 * KD), ch = idx - row * (4 * KD);
-    const uint32_t swz = INT8 || g < 2 * KD ? swz_k<KD>(row) : swz_v<KD>(row);
-    voff[i] = (row & 15u) * c.slot_bytes + ((ch ^ swz) * 16);
+    const uint32_t swz = INT8 ? swz_i8<KD>(row) : g < 2 * KD ? swz_k<KD>(row) : swz_v<KD>(row);
+    voff[i] = (row & 15u) * (2 * DIM) + ((ch ^ swz) * 16);
   }
   const char* head_base = c.pages + (uint64_t)h * c.head_bytes;
   // Page numbers come through the scalar cache (the constant address space makes the compiler load them so): a vector
@@ -319,8 +357,8 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
     x.inside = x.inside && x.page < c.num_pages;
     if (!x.inside) x.page = x.slot = 0;
   };
-  auto base_of = [&](const Block& x) { return head_base + (uint64_t)x.page * c.page_bytes + (uint64_t)x.slot * c.slot_bytes; };
-  auto key_of = [&](int32_t turn) { return k_begin + 32 * (int32_t)(kw + KW * turn); };
+  auto base_of = [&](const Block& x) { return uniform(head_base + (uint64_t)x.page * c.page_bytes + (uint64_t)x.slot * c.slot_bytes); };
+  auto key_of = [&](int32_t turn) { return k_begin + KEYS * (int32_t)(kw + KW * turn); };
   // starts the transfers of a turn's 32 keys; returns which halves are inside the cache
   auto issue = [&](Block x0, Block x1, uint32_t stage) -> uint32_t {
     settle_block(x0);
@@ -353,99 +391,186 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
     for (int d = 0; d < 2 * KD; d++) acc[t][d] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto compute = [&](int32_t turn, uint32_t stage, uint32_t inside) {
+  // where a lane reads: its part of the addresses (a 16-row half and a stage are constants on top)
+  uint32_t k_at[KD], v_at[2 * KD];
+#pragma unroll
+  for (int x = 0; x < KD; x++) {
+    if constexpr (RAW8) k_at[x] = lj * (2 * DIM) + (((2 * x + (lc >> 1)) ^ swz_i8<KD>(lj)) * 16) + (lc & 1u) * 8;
+    else k_at[x] = lj * (2 * DIM) + (((4 * x + lc) ^ swz_k<KD>(lj)) * 16);
+  }
+#pragma unroll
+  for (int d = 0; d < 2 * KD; d++) {
+    if constexpr (RAW8) {
+      const uint32_t row = 16 * (lj >> 3) + 4 * lc + ((lj >> 1) & 3u);
+      v_at[d] = row * (2 * DIM) + (((2 * KD + d) ^ swz_i8<KD>(row)) * 16) + (lj & 1u) * 8;
+    } else {
+      const uint32_t row = 4 * lc + (lj >> 2);
+      v_at[d] = 2 * KEYS * DIM + row * (2 * DIM) + (((2 * d + ((lj & 3u) >> 1)) ^ swz_v<KD>(row)) * 16) + (lj & 1u) * 8;
+    }
+  }
+
+  // One tile of KEYS keys. kv: the staged rows (f16, or int8 as they came); pairs: their scales; inside: which 16-key
+  // blocks are in the cache.
+  auto compute = [&](int32_t turn, uint32_t at, uint32_t pairs_at, uint32_t inside) {
+    constexpr int H = 2 * NS;  // 16-key blocks
     const int32_t pos = key_of(turn);
     if (pos >= k_end) return;
-    const char* kv = lds + stage * Shape::STAGE + kw * Shape::PART;
-    f4 s[QT][2];
+    const char* kv = lds + at;
+    const char* pairs = lds + at + pairs_at;
+    const bool edge = pos + KEYS > full || inside != (1u << H) - 1u;  // some row does not see some key
+    f4 s[QT][H];
 #pragma unroll
-    for (int t = 0; t < QT; t++) s[t][0] = s[t][1] = f4{0.f, 0.f, 0.f, 0.f};
-    static_for<2>([&](auto half_) {
-      constexpr int half = decltype(half_)::value;
-      const uint32_t row = 16 * half + lj;
+    for (int t = 0; t < QT; t++)
 #pragma unroll
-      for (int x = 0; x < KD; x++) {
+      for (int half = 0; half < H; half++) s[t][half] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < KD; x++)
+      static_for<H>([&](auto half_) {
+        constexpr int half = decltype(half_)::value;
         h8 k;
-        if constexpr (INT8) {  // 8 bytes: half of a chunk
-          const uint32_t ch = 2 * x + (lc >> 1);
-          k = widen_i8(*reinterpret_cast<const u32x2*>(kv + row * (2 * DIM) + ((ch ^ swz_k<KD>(row)) * 16) + (lc & 1u) * 8));
+        if constexpr (RAW8) {  // 8 bytes: half of a chunk
+          constexpr uint32_t FLIP = 16u * (swz_i8<KD>(16));
+          k = widen_i8(*reinterpret_cast<const u32x2*>(kv + (half ? (k_at[x] ^ FLIP) + 32 * DIM : k_at[x])));
         } else {
-          k = *reinterpret_cast<const h8*>(kv + row * (2 * DIM) + (((4 * x + lc) ^ swz_k<KD>(row)) * 16));
+          k = *reinterpret_cast<const h8*>(kv + k_at[x] + half * 32 * DIM);
         }
 #pragma unroll
         for (int t = 0; t < QT; t++) s[t][half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[t][x], s[t][half], 0, 0, 0);
-      }
-    });
-    // scales: log2 units of the scores, and what the values' rows weigh
-    float ks[2][4], vs[2][4];
-    if constexpr (INT8) {
-      const char* pairs = lds + stage * Shape::STAGE + KW * Shape::PART + kw * Shape::SCALES;
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
+      });
+    // int8: the keys' scales
+    auto scale_of = [&](int half, bool value, float* out) {  // of the lane's four keys of a block
+      if constexpr (RAW8) {
         const u32x4 four = *reinterpret_cast<const u32x4*>(pairs + 64 * half + 16 * lc);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const h2 pair = as_h2(four[i]);
-          ks[half][i] = (float)pair.x * p.scale_log2;
-          vs[half][i] = (float)pair.y * LIFT;
+          out[i] = value ? (float)pair.y : (float)pair.x * p.scale_log2;
         }
+      } else {
+        const f4 four = *reinterpret_cast<const f4*>(pairs + (value ? 4 * KEYS : 0) + 64 * half + 16 * lc);
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = four[i];
+      }
+    };
+    if constexpr (INT8) {
+#pragma unroll
+      for (int half = 0; half < H; half++) {
+        float ks[4];
+        scale_of(half, false, ks);
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[t][half][i] *= ks[i];
       }
     }
-    const bool edge = pos + 32 > full || inside != 3u;
-    h8 pf[QT];
+    const float units = INT8 ? 1.f : p.scale_log2;  // s * units: the scores in log2 units
+    uint64_t there = ~0ull;
+    if (edge) {
+      there = 0;
+#pragma unroll
+      for (int half = 0; half < H; half++) there |= inside >> half & 1u ? 0xFFFFull << (16 * half) : 0ull;
+    }
+    // int8: a scale that is no number (of a slot nobody wrote, say) must not enter as 0 * inf where it is not seen
+    uint32_t odd = 0;
+    if constexpr (INT8) {
+      if (edge) {
+        bool any = false;
+#pragma unroll
+        for (int half = 0; half < H; half++) {
+          float vs[4];
+          scale_of(half, true, vs);
+#pragma unroll
+          for (int i = 0; i < 4; i++) any |= !(fabsf(vs[i]) <= 65504.f);
+        }
+        odd = __any(any) ? 1u : 0u;
+      }
+      odd = __builtin_amdgcn_readfirstlane(odd);
+      asm volatile("" : "+s"(odd));  // a condition of its own: tied to `edge` the compiler doubles the code behind it
+    }
+    h8 pf[QT][NS];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      float x[2][4];
-#pragma unroll
-      for (int half = 0; half < 2; half++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[half][i] = s[t][half][i] * (INT8 ? ks[half][i] : p.scale_log2);
-      uint32_t seen = ~0u;
+      uint32_t seen[NS];  // bit 16*half + i of a 32-key part: the lane's row sees key 16*half + 4*lc + i of it
       if (edge) {
-        seen = visible_bits(pos, context, limit[t], words[t], a.mask_words) & (inside & 1u ? ~0u : 0xFFFF0000u) & (inside & 2u ? ~0u : 0x0000FFFFu);
-        seen >>= 4 * lc;
+        const uint64_t bits = visible_bits(pos, context, limit[t], tree ? a.tree_mask + (size_t)token[t] * a.mask_words : nullptr, a.mask_words) & there;
 #pragma unroll
-        for (int half = 0; half < 2; half++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) x[half][i] = seen >> (16 * half + i) & 1u ? x[half][i] : -INFINITY;
+        for (int n = 0; n < NS; n++) seen[n] = (uint32_t)(bits >> (32 * n)) >> (4 * lc);
       }
-      float most = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-      if (__any(most > m[t] + THR)) {
-        const float next = fmaxf(m[t], across_groups_max(most));
+      auto sees = [&](int half, int i) { return (seen[half / 2] >> (16 * (half & 1) + i) & 1u) != 0; };
+      // probabilities against the reference value as it stands; where one of them passes CAP the reference moves and they
+      // are taken again
+      float e[H][4];
+      auto weigh = [&]() {
+        const float down = m[t] - LIFT;
+#pragma unroll
+        for (int half = 0; half < H; half++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            e[half][i] = __builtin_amdgcn_exp2f(INT8 ? s[t][half][i] - down : __builtin_fmaf(s[t][half][i], units, -down));
+        if (edge) {
+#pragma unroll
+          for (int half = 0; half < H; half++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[half][i] = sees(half, i) ? e[half][i] : 0.f;
+        }
+      };
+      weigh();
+      float most = 0.f;
+#pragma unroll
+      for (int half = 0; half < H; half++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) most = fmaxf(most, e[half][i]);
+      if (__any(most > CAP)) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int half = 0; half < H; half++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x = s[t][half][i] * units;
+            top = fmaxf(top, !edge || sees(half, i) ? x : -INFINITY);
+          }
+        const float next = fmaxf(m[t], across_groups_max(top));
         const float keep = __builtin_amdgcn_exp2f(m[t] - next);
         m[t] = next;
         l[t] *= keep;
 #pragma unroll
         for (int d = 0; d < 2 * KD; d++) acc[t][d] *= keep;
+        weigh();
       }
 #pragma unroll
-      for (int half = 0; half < 2; half++)
+      for (int half = 0; half < H; half++) {
+        float vs[4] = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (INT8) scale_of(half, true, vs);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float e = __builtin_amdgcn_exp2f(x[half][i] - m[t]);
-          l[t] += e;
-          float w = e * (INT8 ? vs[half][i] : LIFT);
-          if (INT8 && edge) w = seen >> (16 * half + i) & 1u ? w : 0.f;  // a scale nobody wrote may be anything
-          pf[t][4 * half + i] = (_Float16)w;
+          l[t] += e[half][i];
+          pf[t][half / 2][4 * (half & 1) + i] = (_Float16)(INT8 ? e[half][i] * vs[i] : e[half][i]);
         }
+      }
+      if (INT8 && odd) {
+#pragma unroll
+        for (int half = 0; half < H; half++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (!sees(half, i)) pf[t][half / 2][4 * (half & 1) + i] = (_Float16)0.f;
+      }
     }
 #pragma unroll
     for (int d = 0; d < 2 * KD; d++) {
-      h8 v;
-      if constexpr (INT8) {
-        const uint32_t row = 16 * (lj >> 3) + 4 * lc + ((lj >> 1) & 3u), ch = 2 * KD + d;
-        const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(kv + row * (2 * DIM) + ((ch ^ swz_k<KD>(row)) * 16) + (lj & 1u) * 8));
-        v = widen_i8(u32x2{(uint32_t)raw.x, (uint32_t)raw.y});
-      } else {
-        const uint32_t ch = 2 * d + ((lj & 3u) >> 1);
-        s16x4 r[2];
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const uint32_t row = 16 * half + 4 * lc + (lj >> 2);
-          r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(kv + 64 * DIM + row * (2 * DIM) + ((ch ^ swz_v<KD>(row)) * 16) + (lj & 1u) * 8));
+      for (int n = 0; n < NS; n++) {
+        h8 v;
+        if constexpr (RAW8) {
+          const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(kv + v_at[d]));
+          v = widen_i8(u32x2{(uint32_t)raw.x, (uint32_t)raw.y});
+        } else {
+          s16x4 r[2];
+#pragma unroll
+          for (int half = 0; half < 2; half++)
+            r[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(kv + v_at[d] + (2 * n + half) * 32 * DIM));
+          v = __builtin_bit_cast(h8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        v = __builtin_bit_cast(h8, __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        if (edge) {
+        if (!INT8 && edge) {
           // An infinity or NaN that nobody sees must not enter as 0 * inf: the product gets a zero, and rows that do
           // see it get it back by its sign.
           u16x8 bits = __builtin_bit_cast(u16x8, v);
@@ -466,7 +591,7 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
             for (int t = 0; t < QT; t++) {
               h8 sees;
 #pragma unroll
-              for (int i = 0; i < 8; i++) sees[i] = pf[t][i] > (_Float16)0.f ? (_Float16)1.f : (_Float16)0.f;
+              for (int i = 0; i < 8; i++) sees[i] = pf[t][n][i] > (_Float16)0.f ? (_Float16)1.f : (_Float16)0.f;
               const f4 zero = {0.f, 0.f, 0.f, 0.f};
               const f4 ups = __builtin_amdgcn_mfma_f32_16x16x32_f16(up, sees, zero, 0, 0, 0);
               const f4 downs = __builtin_amdgcn_mfma_f32_16x16x32_f16(down, sees, zero, 0, 0, 0);
@@ -478,15 +603,19 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
             }
           }
         }
-      }
 #pragma unroll
-      for (int t = 0; t < QT; t++) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[t], acc[t][d], 0, 0, 0);
+        for (int t = 0; t < QT; t++) acc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[t][n], acc[t][d], 0, 0, 0);
+      }
     }
   };
 
   // ---- the pipeline
   uint32_t halves = 0;  // two bits for each stage in flight, the oldest lowest
   if constexpr (RW == 1) {  // a wave's keys are its own: no barrier; a stage is filled again as soon as it has been used
+#pragma unroll
+    for (int i = 0; i < KD; i++) k_at[i] += kw * Shape::PART;
+#pragma unroll
+    for (int i = 0; i < 2 * KD; i++) v_at[i] += kw * Shape::PART;
 #pragma unroll
     for (int i = 0; i < ST; i++)
       if (i < turns) halves |= issue(block_at(key_of(i)), block_at(key_of(i) + 16), i) << (2 * i);
@@ -495,12 +624,12 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
       const Block x0 = block_at(key_of(turn + ST)), x1 = block_at(key_of(turn + ST) + 16);
       if (turn + ST - 1 < turns) wait_vm<(ST - 1) * DMA>();
       else wait_vm<0>();
-      compute(turn, stage, halves & 3u);
+      compute(turn, stage * Shape::STAGE, KW * Shape::PART + kw * Shape::SCALES, halves & 3u);
       halves >>= 2;
       wait_lgkm<0>();
       if (turn + ST < turns) halves |= issue(x0, x1, stage) << (2 * (ST - 1));
     }
-  } else {
+  } else if constexpr (!Shape::WIDEN) {
 #pragma unroll
     for (int i = 0; i < ST - 1; i++)
       if (i < turns) halves |= issue(block_at(key_of(i)), block_at(key_of(i) + 16), i) << (2 * i);
@@ -510,46 +639,113 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
       else wait_vm<0>();
       wg_barrier();  // everybody's transfers of this stage have landed, everybody has left the stage before
       if (turn + ST - 1 < turns) halves |= issue(x0, x1, (turn + ST - 1) % ST) << (2 * (ST - 1));
-      compute(turn, turn % ST, halves & 3u);
+      compute(turn, turn % ST * Shape::STAGE, 0u, halves & 3u);
       halves >>= 2;
       wait_lgkm<0>();
+    }
+  } else {
+    // int8 rows that several waves share: each wave fetches its part of a tile into registers a turn ahead and widens it
+    // for all, so the products read f16 tiles.
+    constexpr uint32_t SIDE = 32 * KD;                      // 16-byte chunks of K (and of V) in the wave's 16 keys
+    constexpr int LOADS = KD;                               // 64 chunks each: K, then V (KD odd: the middle one holds both)
+    uint32_t from[LOADS], to_at[LOADS], key[LOADS];
+    bool is_v[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      const uint32_t u = 64 * i + lane;
+      is_v[i] = KD % 2 == 0 ? i >= KD / 2 : u >= SIDE;
+      const uint32_t w = is_v[i] ? u - SIDE : u, row = w / (2 * KD), ch = w - row * (2 * KD);
+      key[i] = row;
+      from[i] = row * (2 * DIM) + (is_v[i] ? DIM : 0) + ch * 16;
+      const uint32_t swz = is_v[i] ? swz_v<KD>(row) : swz_k<KD>(row);
+      to_at[i] = (is_v[i] ? 2 * KEYS * DIM : 0) + (16 * rw + row) * (2 * DIM) + ((2 * ch) ^ swz) * 16;
+    }
+    u32x4 raw[LOADS];
+    uint32_t pair;  // of key lane % 16
+    bool have;
+    auto fetch = [&](Block x) {
+      settle_block(x);
+      have = x.inside;
+      const char* base = base_of(x);
+      const char* scales = uniform(reinterpret_cast<const char*>(c.scales + kv_scale_index(c, x.page, h, x.slot, 0)));
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) raw[i] = *reinterpret_cast<const u32x4*>(base + from[i]);
+      pair = *reinterpret_cast<const uint32_t*>(scales + 4u * lj);
+    };
+    auto widen = [&](int32_t turn) {
+      char* to = lds + (turn & 1) * Shape::WIDE;
+      const h2 scales = as_h2(pair);
+      const _Float16 sv = scales.y, power = power_of(__builtin_bit_cast(uint16_t, sv));
+      if (lane < 16) {
+        *reinterpret_cast<float*>(to + Shape::PAIRS + 4 * (16 * rw + lane)) = (float)scales.x * p.scale_log2;
+        *reinterpret_cast<float*>(to + Shape::PAIRS + 4 * (KEYS + 16 * rw + lane)) = (float)sv / (float)power;
+      }
+      if (lane == 0) *reinterpret_cast<uint32_t*>(to + Shape::FLAGS + 4 * rw) = have ? 1u << rw : 0u;
+      const int power_bits = (int)as_u32(h2{power, power});
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        h8 lo = widen_i8(u32x2{raw[i].x, raw[i].y}), hi = widen_i8(u32x2{raw[i].z, raw[i].w});
+        if (KD % 2 != 0 || i >= KD / 2) {
+          h2 f = as_h2((uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * key[i]), power_bits));
+          if (KD % 2 != 0 && !is_v[i]) f = h2{(_Float16)1.f, (_Float16)1.f};
+          lo *= h8{f.x, f.x, f.x, f.x, f.x, f.x, f.x, f.x};
+          hi *= h8{f.x, f.x, f.x, f.x, f.x, f.x, f.x, f.x};
+        }
+        *reinterpret_cast<h8*>(to + to_at[i]) = lo;
+        *reinterpret_cast<h8*>(to + (to_at[i] ^ 16u)) = hi;
+      }
+    };
+    if (turns) {
+      auto block_of = [&](int32_t turn) { return block_at(key_of(turn) + 16 * (int32_t)rw); };
+      fetch(block_of(0));
+      Block ahead = block_of(1);
+      widen(0);
+      fetch(ahead);
+      ahead = block_of(2);
+      for (int32_t turn = 0; turn < turns; turn++) {
+        wait_lgkm<0>();
+        wg_barrier();  // this tile is widened; everybody has left the one before
+        if (turn + 1 < turns) widen(turn + 1);
+        fetch(ahead);  // past the end: rows that exist, not looked at
+        ahead = block_of(turn + 3);
+        const u32x4 flags = *reinterpret_cast<const u32x4*>(lds + (turn & 1) * Shape::WIDE + Shape::FLAGS);
+        compute(turn, (turn & 1) * Shape::WIDE, Shape::PAIRS, __builtin_amdgcn_readfirstlane(flags.x | flags.y | flags.z | flags.w));
+      }
     }
   }
 
   // ---- join the key waves, then either the result or a partial one
 #pragma unroll
   for (int t = 0; t < QT; t++) l[t] = across_groups_sum(l[t]);
-  const bool last = parts == 1;
-  auto store4 = [&](uint32_t row, uint32_t d, f4 v, float total) {  // four dims of a row; v is times LIFT
-    if (last) {
-      const uint32_t i = row / p.group;
-      const float inv = total > 0.f || total != total ? 1.0f / (total * LIFT) : 0.f;
-      h4 o;
+  auto finish4 = [&](uint32_t row, uint32_t d, f4 v, float total) {  // four dims of a row; v and total are times 2^LIFT
+    const uint32_t i = row / p.group;
+    const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+    h4 o;
 #pragma unroll
-      for (int x = 0; x < 4; x++) o[x] = narrow_f32(v[x] * inv);
-      *reinterpret_cast<h4*>(a.out + (size_t)(start + i) * a.out_stride + (size_t)(h * p.group + (row - i * p.group)) * DIM + d) = o;
-    } else {
-      const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits + split;
-      *reinterpret_cast<f4*>(p.partial + at * DIM + d) = v;
-    }
+    for (int x = 0; x < 4; x++) o[x] = narrow_f32(v[x] * inv);
+    *reinterpret_cast<h4*>(a.out + (size_t)(start + i) * a.out_stride + (size_t)(h * p.group + (row - i * p.group)) * DIM + d) = o;
   };
-  auto store_row = [&](uint32_t row, float top, float total) {
-    if (last) {
-      const uint32_t i = row / p.group;
-      if (a.lse) a.lse[(size_t)(start + i) * a.heads + h * p.group + (row - i * p.group)] = total > 0.f || total != total ? (top + __log2f(total)) * 0.69314718055994531f : -INFINITY;
-    } else {
-      const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits + split;
-      p.partial_ml[at] = make_float2(top, total);
-    }
+  auto finish_row = [&](uint32_t row, float top, float total) {
+    const uint32_t i = row / p.group;
+    if (a.lse) a.lse[(size_t)(start + i) * a.heads + h * p.group + (row - i * p.group)] = total > 0.f || total != total ? (top - LIFT + __log2f(total)) * 0.69314718055994531f : -INFINITY;
   };
+  // where a row's partial results of split 0 are; the other splits follow
+  auto partial_at = [&](uint32_t row) { return ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits; };
   if constexpr (KW == 1) {
 #pragma unroll
     for (int t = 0; t < QT; t++) {
       const uint32_t row = wave_row + 16 * t + lj;
       if (row < rows) {
-        if (lc == 0) store_row(row, m[t], l[t]);
+        if (parts == 1) {
+          if (lc == 0) finish_row(row, m[t], l[t]);
 #pragma unroll
-        for (int d = 0; d < 2 * KD; d++) store4(row, 16 * d + 4 * lc, acc[t][d], l[t]);
+          for (int d = 0; d < 2 * KD; d++) finish4(row, 16 * d + 4 * lc, acc[t][d], l[t]);
+        } else {  // attention_join_kernel adds the parts
+          const size_t at = partial_at(row) + split;
+          if (lc == 0) p.partial_ml[at] = make_float2(m[t], l[t]);
+#pragma unroll
+          for (int d = 0; d < 2 * KD; d++) *reinterpret_cast<f4*>(p.partial + at * DIM + 16 * d + 4 * lc) = acc[t][d];
+        }
       }
     }
   } else {
@@ -583,8 +779,62 @@ __global__ __launch_bounds__(64 * RW * KW, KD <= 4 ? 2 : 1) void attention_mfma_
         total += ml[k * ROWS + local].y * __builtin_amdgcn_exp2f(ml[k * ROWS + local].x - top);
         v += *reinterpret_cast<const f4*>(joined + (k * ROWS + local) * Shape::PITCH + d);
       }
-      store4(row, d, v, total);
-      if (d == 0) store_row(row, top, total);
+      if (parts == 1) {
+        finish4(row, d, v, total);
+        if (d == 0) finish_row(row, top, total);
+      } else {
+        const size_t at = partial_at(row) + split;
+        put2(p.partial + at * DIM + d, v.x, v.y);
+        put2(p.partial + at * DIM + d + 2, v.z, v.w);
+        if (d == 0) put2(reinterpret_cast<float*>(p.partial_ml + at), top, total);
+      }
+    }
+    if (parts == 1) return;
+    // The workgroup that arrives last adds the parts, in their order. Partial results go past the caches that the XCDs do
+    // not share (relaxed device-scope stores and loads), every wave waits for its own stores before the barrier, and one
+    // thread counts the arrival; nobody waits for another workgroup.
+    uint32_t* flag = reinterpret_cast<uint32_t*>(lds);
+    wait_vm<0>();
+    __syncthreads();
+    const uint32_t group_id = ((uint32_t)blockIdx.y * a.sequences + b) * c.kv_heads + h;
+    if (tid == 0) *flag = __hip_atomic_fetch_add(p.arrivals + group_id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const bool last = *flag == parts - 1;
+    __syncthreads();
+    if (!last) return;
+    if (tid == 0) __hip_atomic_store(p.arrivals + group_id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t here = min(rows - row0, (uint32_t)ROWS);
+    float2* weights = reinterpret_cast<float2*>(lds);  // [row][split]
+    for (uint32_t i = tid; i < here * parts; i += 64 * RW * KW) {
+      const uint32_t local = i / parts, s = i - local * parts;
+      weights[local * parts + s] = get2(reinterpret_cast<const float*>(p.partial_ml + partial_at(row0 + local) + s));
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < here * (DIM / 4); i += 64 * RW * KW) {
+      const uint32_t local = i / (DIM / 4), d = (i - local * (DIM / 4)) * 4, row = row0 + local;
+      const float* from = p.partial + partial_at(row) * DIM + d;
+      const float2* w = weights + local * parts;
+      float top = NOTHING, total = 0.f;
+      for (uint32_t s = 0; s < parts; s++) top = fmaxf(top, w[s].x);
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s0 = 0; s0 < parts; s0 += 16) {
+        float2 lo[16], hi[16];
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++) {
+          const uint32_t s = min(s0 + k, parts - 1);
+          lo[k] = get2(from + (size_t)s * DIM);
+          hi[k] = get2(from + (size_t)s * DIM + 2);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 16; k++)
+          if (s0 + k < parts) {
+            const float f = __builtin_amdgcn_exp2f(w[s0 + k].x - top);
+            total += w[s0 + k].y * f;
+            v += f4{lo[k].x, lo[k].y, hi[k].x, hi[k].y} * f;
+          }
+      }
+      finish4(row, d, v, total);
+      if (d == 0) finish_row(row, top, total);
     }
   }
 }
@@ -611,38 +861,62 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
   const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits;
   const float* acc = p.partial + at * c.head_dim;
   const float2* ml = p.partial_ml + at;
+  // a lane takes four dims of every `ways`-th split; eight of them are asked for before the weights are known
+  const uint32_t quads = c.head_dim / 4, ways = 64u / quads, way = lane / quads, d = (lane - way * quads) * 4;
+  constexpr uint32_t BATCH = 8;
+  f4 x[BATCH];
+  auto batch = [&](uint32_t s1) {
+#pragma unroll
+    for (uint32_t k = 0; k < BATCH; k++) {
+      const uint32_t s = s1 + k * ways + way;
+      x[k] = s < parts && way < ways ? *reinterpret_cast<const f4*>(acc + (size_t)s * c.head_dim + d) : f4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  batch(0);
   float top = NOTHING;
   for (uint32_t s = lane; s < parts; s += 64u) top = fmaxf(top, ml[s].x);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};  // dims lane, lane + 64, ..
+  float total = 0.f;
+  f4 v = {0.f, 0.f, 0.f, 0.f};
   for (uint32_t s0 = 0; s0 < parts; s0 += 64u) {
     const uint32_t here = min(parts - s0, 64u);
     const float2 mine = lane < here ? ml[s0 + lane] : make_float2(NOTHING, 0.f);
     const float w = lane < here ? __builtin_amdgcn_exp2f(mine.x - top) : 0.f;
     total += mine.y * w;
-#pragma unroll 8
-    for (uint32_t s = 0; s < here; s++) {
-      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), (int)s));
+    for (uint32_t s1 = 0; s1 < here; s1 += BATCH * ways) {
+      if (s0 + s1) batch(s0 + s1);
 #pragma unroll
-      for (uint32_t k = 0; k < 4; k++)
-        if (lane + 64u * k < c.head_dim) v[k] += acc[(size_t)(s0 + s) * c.head_dim + lane + 64u * k] * ws;
+      for (uint32_t k = 0; k < BATCH; k++) {
+        const uint32_t s = s1 + k * ways + way;
+        const float ws = __shfl(w, (int)min(s, 63u));
+        if (s < 64u) v += x[k] * ws;
+      }
     }
   }
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  const float inv = total > 0.f || total != total ? 1.0f / (total * lift) : 0.f;
-  const uint32_t i = row / p.group, head = h * p.group + (row - i * p.group);
-  _Float16* out = a.out + (size_t)(start + i) * a.out_stride + (size_t)head * c.head_dim;
+  f4 sum = v;
+  for (uint32_t k = 1; k < ways; k++) {
+    f4 other;
 #pragma unroll
-  for (uint32_t k = 0; k < 4; k++)
-    if (lane + 64u * k < c.head_dim) out[lane + 64u * k] = narrow_f32(v[k] * inv);
-  if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top + __log2f(total)) * 0.69314718055994531f : -INFINITY;
+    for (int x = 0; x < 4; x++) other[x] = __shfl(v[x], (int)min(lane + k * quads, 63u));
+    sum += other;  // of use in the first way only, where the ways are added in their order
+  }
+  const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
+  const uint32_t i = row / p.group, head = h * p.group + (row - i * p.group);
+  if (way == 0) {
+    h4 o;
+#pragma unroll
+    for (int x = 0; x < 4; x++) o[x] = narrow_f32(sum[x] * inv);
+    *reinterpret_cast<h4*>(a.out + (size_t)(start + i) * a.out_stride + (size_t)head * c.head_dim + d) = o;
+  }
+  if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top - lift + __log2f(total)) * 0.69314718055994531f : -INFINITY;
 }
 
 // What the matrix-core kernel takes: whole 64-byte units of a head, pages of whole 16-key blocks, 16-byte rows.
 bool mfma_takes(const AttentionArgs& a) {
   const KvView& c = a.cache;
   const uint32_t kd = c.head_dim / 32;
-  if (c.head_dim % 32 || !(kd == 2 || kd == 3 || kd == 4 || kd == 8)) return false;
+  if (c.head_dim % 32 || c.slot_bytes != 2 * c.head_dim || !(kd == 2 || kd == 3 || kd == 4 || kd == 8)) return false;
   if (c.page_size % 16 || !c.num_pages || !a.max_kv) return false;
   const uint64_t at = reinterpret_cast<uint64_t>(c.pages) | c.page_bytes | c.head_bytes | c.side_bytes | c.slot_bytes;
   if (at % 16 || reinterpret_cast<uint64_t>(c.scales) % 4) return false;
@@ -657,6 +931,9 @@ struct MfmaPlan {
   uint32_t rows, row_tiles, splits, chunk;
   size_t partial_bytes, bytes;
 };
+#ifndef ATTN_LEAST
+#define ATTN_LEAST 2u
+#endif
 #ifndef ATTN_KW1
 #define ATTN_KW1 2
 #endif
@@ -667,20 +944,18 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   const bool wide = a.cache.head_dim > 128;
   if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = wide ? 2 : ATTN_KW1;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
-  else g.qt = 2, g.rw = 4, g.kw = 1;
+  else g.qt = rows <= 64 || wide ? 1 : 2, g.rw = 4, g.kw = 1;
   g.rows = 16 * g.qt * g.rw;
   g.row_tiles = (uint32_t)((rows + g.rows - 1) / g.rows);
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
   // enough workgroups for a few rounds of the CUs, none with less than four turns of its waves
-#ifndef ATTN_WANT
-#define ATTN_WANT 1024
-#endif
-  const uint64_t want = ATTN_WANT;
-  const uint32_t least = 32u * g.kw * 4u;
+  const uint64_t want = g.rw == 1 ? 2048 : a.sequences == 1 ? 512 : 1024;
+  const uint32_t unit = std::max(32u * g.kw, 64u), least = unit * (g.kw > 1 ? ATTN_LEAST : 4u);
   uint64_t splits = (want + groups - 1) / groups;
-  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (a.max_kv + least - 1) / least));
-  g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + 32 * g.kw - 1) / (32 * g.kw) * (32 * g.kw));
+  splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, (a.max_kv + least - 1) / least, (uint64_t)MOST_SPLITS}));
+  g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + unit - 1) / unit * unit);
   g.splits = (a.max_kv + g.chunk - 1) / g.chunk;
+  static_assert(ZTVM_ATTENTION_ARRIVALS >= 2048, "a counter for every row tile that is split");
   if (g.splits > 1) {
     const uint64_t n = (uint64_t)a.sequences * a.heads * a.max_query * g.splits;
     g.partial_bytes = n * a.cache.head_dim * 4;
@@ -689,39 +964,41 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   return g;
 }
 
-template <int KD, bool INT8, int QT, int RW, int KW>
+template <int KD, bool INT8, int QT, int RW, int KW, int NS>
 hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t s) {
-  using Shape = MfmaShape<KD, INT8, QT, RW, KW>;
-  auto kernel = attention_mfma_kernel<KD, INT8, QT, RW, KW>;
+  using Shape = MfmaShape<KD, INT8, QT, RW, KW, NS>;
+  auto kernel = attention_mfma_kernel<KD, INT8, QT, RW, KW, NS>;
   if (Shape::LDS > 64 * 1024) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Shape::LDS);
   const dim3 grid(p.a.sequences * p.a.cache.kv_heads * g.splits, g.row_tiles);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * RW * KW), Shape::LDS, s, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || g.splits == 1) return e;
+  if (e != hipSuccess || g.splits == 1 || KW > 1) return e;
   const uint32_t units = std::min(p.a.max_query, p.a.tokens) * p.a.heads;
-  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, INT8 ? 16.f : 512.f);
+  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
   return hipGetLastError();
 }
 template <int KD, bool INT8>
 hipError_t launch_mfma_dim(const MfmaParams& p, const MfmaPlan& g, hipStream_t s) {
   constexpr int KW = KD > 4 ? 2 : 4;
-  if (g.rw == 4) return launch_mfma_shape<KD, INT8, 2, 4, 1>(p, g, s);
-  if (g.qt == 2) return launch_mfma_shape<KD, INT8, 2, 1, KW>(p, g, s);
-  return launch_mfma_shape<KD, INT8, 1, 1, (KD > 4 ? 2 : ATTN_KW1)>(p, g, s);
+  constexpr int NS = INT8 ? 2 : 1;
+  if (g.rw == 4 && g.qt == 2) return launch_mfma_shape<KD, INT8, (KD > 4 ? 1 : 2), 4, 1, NS>(p, g, s);
+  if (g.rw == 4) return launch_mfma_shape<KD, INT8, 1, 4, 1, NS>(p, g, s);
+  if (g.qt == 2) return launch_mfma_shape<KD, INT8, 2, 1, KW, 1>(p, g, s);
+  return launch_mfma_shape<KD, INT8, 1, 1, (KD > 4 ? 2 : ATTN_KW1), 1>(p, g, s);
 }
 
 }  // namespace
 
 size_t attention_scratch_bytes(const AttentionArgs& a) { return mfma_takes(a) ? mfma_plan(a).bytes : 0; }
 
-hipError_t launch_attention(const AttentionArgs& a, void* scratch, hipStream_t s) {
+hipError_t launch_attention(const AttentionArgs& a, void* scratch, uint32_t* arrivals, hipStream_t s) {
   if (!mfma_takes(a)) {
     hipLaunchKernelGGL(attention_any_kernel, dim3(a.tokens, a.heads), dim3(256), 0, s, a);
     return hipGetLastError();
   }
   const MfmaPlan g = mfma_plan(a);
-  MfmaParams p{a, static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + g.partial_bytes), g.splits, g.chunk,
-               a.heads / a.cache.kv_heads, fabsf(a.scale) * 1.4426950408889634f, a.scale < 0.f};
+  MfmaParams p{a, static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + g.partial_bytes), arrivals, g.splits, g.chunk,
+               a.heads / a.cache.kv_heads, std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f), a.scale < 0.f};  // never 0: a masked score is -inf times it
   auto by_format = [&](auto kd) {
     constexpr int KD = decltype(kd)::value;
     return a.cache.int8 ? launch_mfma_dim<KD, true>(p, g, s) : launch_mfma_dim<KD, false>(p, g, s);

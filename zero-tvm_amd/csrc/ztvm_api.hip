@@ -72,7 +72,7 @@ struct ztvm_ctx {
   // context, which keep its addresses alive (scratch_pool.h).
   std::shared_ptr<DevicePool> scratch;
   void* static_scratch = nullptr;  // this device's copy of the file-scope array above
-  uint32_t* gemm_counters = nullptr;  // arrival counters of the tile GEMM's k split: zero between launches
+  uint32_t* gemm_counters = nullptr;  // arrival counters of the tile GEMM's k split, then of attention's splits: zero between launches
   std::string err;
   hipDeviceProp_t prop;
 };
@@ -421,8 +421,8 @@ int ztvm_create(int device, ztvm_ctx** out) {
   }
   c->scratch = std::make_shared<DevicePool>(DeviceAlloc{device});
   if (!c->scratch->reserve(4u << 20)) return fail(nullptr, ZTVM_E_HIP, "ztvm_create: no device memory for the scratch buffer");
-  HIP_TRY(nullptr, hipMalloc(reinterpret_cast<void**>(&c->gemm_counters), ZTVM_GEMM_SPLIT_TILES * sizeof(uint32_t)));
-  HIP_TRY(nullptr, hipMemset(c->gemm_counters, 0, ZTVM_GEMM_SPLIT_TILES * sizeof(uint32_t)));
+  HIP_TRY(nullptr, hipMalloc(reinterpret_cast<void**>(&c->gemm_counters), (ZTVM_GEMM_SPLIT_TILES + ZTVM_ATTENTION_ARRIVALS) * sizeof(uint32_t)));
+  HIP_TRY(nullptr, hipMemset(c->gemm_counters, 0, (ZTVM_GEMM_SPLIT_TILES + ZTVM_ATTENTION_ARRIVALS) * sizeof(uint32_t)));
   HIP_TRY(nullptr, hipDeviceSynchronize());  // the fill runs on the null stream, which the context's stream does not wait for
   g.c = nullptr;
   *out = c;
@@ -965,7 +965,7 @@ int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
     rc = scratch_for(ctx, need, &scratch);
     if (rc) return rc;
   }
-  HIP_TRY(ctx, launch_attention(a, scratch, ctx->stream));
+  HIP_TRY(ctx, launch_attention(a, scratch, ctx->gemm_counters + ZTVM_GEMM_SPLIT_TILES, ctx->stream));
   return ZTVM_OK;
 }
 
