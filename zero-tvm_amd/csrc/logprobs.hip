@@ -181,122 +181,149 @@ __global__ __launch_bounds__(256) void logits_segments_kernel(const LogprobsArgs
 // value and id of a candidate as one number: larger is better, ties to the lower id
 __device__ __forceinline__ unsigned long long rank_key(float v, uint32_t id) { return (unsigned long long)order_of(v) << 32 | (uint32_t)~id; }
 
-template <class T>
-__global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p, const SegmentStats* all, uint32_t segments, float c) {
-  constexpr uint32_t N = per_load<T>;
-  __shared__ float red[3][4];
+// the logit that has this place in the order
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return order ? __builtin_bit_cast(float, order & 0x80000000u ? order & 0x7FFFFFFFu : ~order) : NAN;
+}
+
+// One workgroup of NT threads per row. A chain of dependent steps bounds it (statistics, their joint maximum, the bound,
+// the neighbourhoods, the places), so everything that does not depend on an earlier step is fetched first, and the
+// neighbourhoods are looked at by all waves at once.
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p, const SegmentStats* all, uint32_t segments, float c) {
+  constexpr uint32_t N = per_load<T>, WAVES = NT / 64;
+  __shared__ float red[3][WAVES];
   __shared__ __align__(16) uint32_t most[256];
-  __shared__ unsigned long long candidates[MAX_CANDIDATES], best[4];
+  __shared__ unsigned long long candidates[MAX_CANDIDATES], best[WAVES];
   __shared__ uint16_t chosen[MAX_HOODS];
-  __shared__ uint32_t count, chosen_count, bound, found;
+  __shared__ uint32_t count, chosen_count, bound;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = blockIdx.x;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
   const uint32_t lead = lead_of(row);
   const SegmentStats* stats = all + (uint64_t)r * segments;
-  if (tid == 0) count = chosen_count = bound = found = 0;
+  const uint32_t K = p.top_ids || p.top_logprobs ? p.top_k : 0;
+  const uint32_t hoods = (lead + p.vocab + hood_size<T> - 1) / hood_size<T>;
+  const bool by_hood = hoods >= K;
+  auto hood_order = [&](uint32_t n) { return order_of(stats[n / HOODS].hood[n % HOODS]); };
+  // what does not wait for anything
+  int32_t token = -1;
+  if (tid == 0 && p.logprob) token = p.tokens[r];
+  SegmentStats first;
+  first.top = -INFINITY;
+  first.total = first.weighted = 0.f;
+  if (tid < segments) first = stats[tid];
+  uint32_t mine = 0;  // the largest of this part of the row, 256 parts
+  if (K && tid < 256u) {
+    if (by_hood) {
+      for (uint32_t n = tid; n < hoods; n += 256u) mine = max(mine, hood_order(n));
+    } else {
+      for (uint32_t i = tid; i < p.vocab; i += 256u) mine = max(mine, order_of((float)row[i]));
+    }
+    most[tid] = mine;
+  }
+  float given = 0.f;
+  const bool in_vocab = token >= 0 && (uint32_t)token < p.vocab;
+  if (in_vocab) given = (float)row[token];
+  if (tid == 0) count = chosen_count = bound = 0;
 
   // ---- the sums
-  float top = -INFINITY;
-  for (uint32_t s = tid; s < segments; s += 256u) top = fmaxf(top, stats[s].top);
+  float top = first.top;
+  for (uint32_t s = tid + NT; s < segments; s += NT) top = fmaxf(top, stats[s].top);
   top = max_of_wave(top);
   if (lane == 0) red[0][wave] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  top = red[0][0];
+#pragma unroll
+  for (uint32_t w = 1; w < WAVES; w++) top = fmaxf(top, red[0][w]);
   const bool low = top == -INFINITY;  // nothing but -inf and NaN
   const float m = low ? 0.f : top;
   float total = 0.f, weighted = 0.f;
-  for (uint32_t s = tid; s < segments; s += 256u) {
-    const SegmentStats v = stats[s];
-    const float d = ((v.top == -INFINITY ? 0.f : v.top) - m) * c;  // e' = e * 2^d, (e*d)' = 2^d * (e*d + d * e)
+  auto add = [&](const SegmentStats& v) {  // e' = e * 2^d, (e*d)' = 2^d * (e*d + d * e)
     const bool none = v.top == -INFINITY;
+    const float d = ((none ? 0.f : v.top) - m) * c;
     const float f = none ? (low ? 1.f : 0.f) : __builtin_amdgcn_exp2f(d);
     total += v.total != v.total ? v.total : v.total * f;
     weighted += v.total != v.total ? v.total : f == 0.f ? 0.f : f * (v.weighted + (none ? 0.f : d) * v.total);
-  }
+  };
+  if (tid < segments) add(first);
+  for (uint32_t s = tid + NT; s < segments; s += NT) add(stats[s]);
   total = sum_of_wave(total);
   weighted = sum_of_wave(weighted);
   if (lane == 0) {
     red[1][wave] = total;
     red[2][wave] = weighted;
   }
+  // ---- meanwhile a bound: the K-th largest of the 256 maxima; at least K logits reach it
+  if (K && tid < 256u) {
+    uint32_t above = 0;  // parts that come before this one
+#pragma unroll 1
+    for (uint32_t w = 0; w < 4; w++) {
+      const uint32_t limit = w < wave ? mine - 1u : mine;  // an equal maximum of a lower part comes first
+      if (w != wave) {
+#pragma unroll 4
+        for (uint32_t j = 64 * w; j < 64 * w + 64; j += 4) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(&most[j]);
+          above += (v.x > limit) + (v.y > limit) + (v.z > limit) + (v.w > limit);
+        }
+      } else {
+#pragma unroll 4
+        for (uint32_t j = 0; j < 64; j += 4) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(&most[64 * w + j]);
+          above += v.x > mine || (v.x == mine && j < lane);
+          above += v.y > mine || (v.y == mine && j + 1 < lane);
+          above += v.z > mine || (v.z == mine && j + 2 < lane);
+          above += v.w > mine || (v.w == mine && j + 3 < lane);
+        }
+      }
+    }
+    if (mine && above == K - 1) bound = mine;
+  }
   __syncthreads();
-  total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  weighted = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+  total = weighted = 0.f;
+#pragma unroll
+  for (uint32_t w = 0; w < WAVES; w++) {
+    total += red[1][w];
+    weighted += red[2][w];
+  }
   constexpr float LN2 = 0.69314718055994531f;
   const bool nothing = low && total == 0.f;  // every logit is -inf (a NaN would be in the sum)
   const float log_total = logf(total);
   auto logp = [&](float v) { return nothing ? -INFINITY : ((v - m) * c) * LN2 - log_total; };
   if (tid == 0) {
-    if (p.logprob) {
-      const int32_t t = p.tokens[r];
-      p.logprob[r] = t >= 0 && (uint32_t)t < p.vocab ? logp((float)row[t]) : -INFINITY;
-    }
+    if (p.logprob) p.logprob[r] = in_vocab ? logp(given) : -INFINITY;
     if (p.entropy) p.entropy[r] = nothing ? 0.f : log_total - weighted / total * LN2;
   }
-  const uint32_t K = p.top_k;
-  if (!K || (!p.top_ids && !p.top_logprobs)) return;
+  if (!K) return;
   auto answer = [&](uint32_t place, unsigned long long key) {
-    const uint32_t id = ~(uint32_t)key;
-    if (p.top_ids) p.top_ids[(size_t)r * K + place] = id;
-    if (p.top_logprobs) p.top_logprobs[(size_t)r * K + place] = logp((float)row[id]);
+    if (p.top_ids) p.top_ids[(size_t)r * K + place] = ~(uint32_t)key;
+    if (p.top_logprobs) p.top_logprobs[(size_t)r * K + place] = logp(value_of((uint32_t)(key >> 32)));
   };
-
-  // ---- a bound: the K-th largest of 256 maxima over disjoint parts of the row; at least K logits reach it
-  const uint32_t hoods = (lead + p.vocab + hood_size<T> - 1) / hood_size<T>;
-  const bool by_hood = hoods >= K;
-  uint32_t mine = 0;
-  if (by_hood) {
-    for (uint32_t n = tid; n < hoods; n += 256u) mine = max(mine, order_of(stats[n / HOODS].hood[n % HOODS]));
-  } else {
-    for (uint32_t i = tid; i < p.vocab; i += 256u) mine = max(mine, order_of((float)row[i]));
-  }
-  most[tid] = mine;
-  __syncthreads();
-  uint32_t above = 0;  // parts that come before this one
-#pragma unroll 1
-  for (uint32_t w = 0; w < 4; w++) {
-    const uint32_t limit = w < wave ? mine - 1u : mine;  // an equal maximum of a lower part comes first
-    if (w != wave) {
-#pragma unroll 4
-      for (uint32_t j = 64 * w; j < 64 * w + 64; j += 4) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(&most[j]);
-        above += (v.x > limit) + (v.y > limit) + (v.z > limit) + (v.w > limit);
-      }
-    } else {
-#pragma unroll 4
-      for (uint32_t j = 0; j < 64; j++) {
-        const uint32_t v = most[64 * w + j];
-        above += v > mine || (v == mine && j < lane);
-      }
-    }
-  }
-  if (mine && above == K - 1) bound = mine;
-  __syncthreads();
   const uint32_t least = bound;
 
   // ---- the neighbourhoods that reach the bound, and every logit of theirs that does
   if (by_hood) {
-    for (uint32_t n = tid; n < hoods; n += 256u)
-      if (order_of(stats[n / HOODS].hood[n % HOODS]) >= least) chosen[atomicAdd(&chosen_count, 1u)] = (uint16_t)n;
+    for (uint32_t n = tid; n < hoods; n += NT)
+      if (hood_order(n) >= least) chosen[atomicAdd(&chosen_count, 1u)] = (uint16_t)n;
     __syncthreads();
   }
   // f(value, id) for every logit that can be among the best
   auto each = [&](auto&& f) {
     if (by_hood) {
-      for (uint32_t k = wave; k < chosen_count; k += 4u) {
-        const uint32_t first = (uint32_t)chosen[k] * hood_size<T>;
+      for (uint32_t k = wave; k < chosen_count; k += WAVES) {
+        const uint32_t from = (uint32_t)chosen[k] * hood_size<T>;
+        float x[2][N];
+#pragma unroll
+        for (uint32_t g = 0; g < 2; g++) load_group(row, lead, p.vocab, from + (g * 64 + lane) * N, 0.f, x[g]);
 #pragma unroll
         for (uint32_t g = 0; g < 2; g++) {
-          float x[N];
-          const uint32_t at = first + (g * 64 + lane) * N;
-          load_group(row, lead, p.vocab, at, 0.f, x);
+          const uint32_t at = from + (g * 64 + lane) * N;
 #pragma unroll
           for (uint32_t i = 0; i < N; i++)
-            if (at + i >= lead && at + i < lead + p.vocab) f(x[i], at + i - lead);
+            if (at + i >= lead && at + i < lead + p.vocab) f(x[g][i], at + i - lead);
         }
       }
     } else {
-      for (uint32_t i = tid; i < p.vocab; i += 256u) f((float)row[i], i);
+      for (uint32_t i = tid; i < p.vocab; i += NT) f((float)row[i], i);
     }
   };
   auto collect = [&](uint32_t from) {  // logits whose order is at least `from`
@@ -309,7 +336,7 @@ __global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p
     __syncthreads();
   };
   auto rank = [&](uint32_t n) {  // places of the first n candidates
-    for (uint32_t i = tid; i < n; i += 256u) {
+    for (uint32_t i = tid; i < n; i += NT) {
       const unsigned long long key = candidates[i];
       uint32_t place = 0;
       for (uint32_t j = 0; j < n; j++) place += candidates[j] > key;
@@ -333,7 +360,7 @@ __global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p
     if (over < K) {
       rank(over);
       uint32_t have = over;
-      for (uint32_t i0 = 0; i0 < p.vocab && have < K; i0 += 256u) {
+      for (uint32_t i0 = 0; i0 < p.vocab && have < K; i0 += NT) {
         const uint32_t i = i0 + tid;
         const bool hit = i < p.vocab && order_of((float)row[i]) == least;
         const unsigned long long ballot = __ballot(hit);
@@ -342,7 +369,7 @@ __global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p
         uint32_t place = have + (uint32_t)__popcll(ballot & ((1ull << lane) - 1ull));
         for (uint32_t w = 0; w < wave; w++) place += most[w];
         if (hit && place < K) answer(place, rank_key((float)row[i], i));
-        have += most[0] + most[1] + most[2] + most[3];
+        for (uint32_t w = 0; w < WAVES; w++) have += most[w];
         __syncthreads();
       }
       return;
@@ -362,7 +389,7 @@ __global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p
     };
     if (reached >= K) each(look);
     else
-      for (uint32_t i = tid; i < p.vocab; i += 256u) look((float)row[i], i);
+      for (uint32_t i = tid; i < p.vocab; i += NT) look((float)row[i], i);
     for (int o = 32; o > 0; o >>= 1) {
       const unsigned long long other = __shfl_xor(key, o);
       key = other > key ? other : key;
@@ -370,7 +397,7 @@ __global__ __launch_bounds__(256) void logits_answer_kernel(const LogprobsArgs p
     if (lane == 0) best[wave] = key;
     __syncthreads();
     last = best[0];
-    for (uint32_t w = 1; w < 4; w++) last = best[w] > last ? best[w] : last;
+    for (uint32_t w = 1; w < WAVES; w++) last = best[w] > last ? best[w] : last;
     __syncthreads();
     if (tid == 0) answer(k, last);
   }
@@ -396,7 +423,9 @@ hipError_t launch_typed(const LogprobsArgs& a, void* scratch, hipStream_t s) {
   const float c = a.inv_temperature * 1.4426950408889634f;
   const uint64_t waves = (uint64_t)a.rows * segments;
   hipLaunchKernelGGL(logits_segments_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, a, stats, segments, c);
-  hipLaunchKernelGGL(logits_answer_kernel<T>, dim3(a.rows), dim3(256), 0, s, a, stats, segments, c);
+  // few rows: as many waves as a row can use; many: as many rows as fit
+  if (a.rows <= 512) hipLaunchKernelGGL((logits_answer_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a, stats, segments, c);
+  else hipLaunchKernelGGL((logits_answer_kernel<T, 256>), dim3(a.rows), dim3(256), 0, s, a, stats, segments, c);
   return hipGetLastError();
 }
 
