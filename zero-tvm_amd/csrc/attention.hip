@@ -955,7 +955,7 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, (a.max_kv + least - 1) / least, (uint64_t)MOST_SPLITS}));
   g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + unit - 1) / unit * unit);
   g.splits = (a.max_kv + g.chunk - 1) / g.chunk;
-  static_assert(ZTVM_ATTENTION_ARRIVALS >= 2048, "a counter for every row tile that is split");
+  static_assert(ZTVM_ARRIVALS >= 2048, "a counter for every row tile that is split");
   if (g.splits > 1) {
     const uint64_t n = (uint64_t)a.sequences * a.heads * a.max_query * g.splits;
     g.partial_bytes = n * a.cache.head_dim * 4;

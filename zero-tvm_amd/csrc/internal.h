@@ -140,8 +140,8 @@ struct LogprobsArgs {
 };
 hipError_t launch_rope_append(const RopeAppendArgs& a, hipStream_t s);
 hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s);
+constexpr uint32_t ZTVM_ARRIVALS = 2048;  // arrival counters a context owns for attention: at most this many split row tiles
 size_t attention_scratch_bytes(const AttentionArgs& a);
-constexpr uint32_t ZTVM_ATTENTION_ARRIVALS = 2048;  // arrival counters a context owns for it: at most this many split row tiles
 hipError_t launch_attention(const AttentionArgs& a, void* scratch, uint32_t* arrivals, hipStream_t s);
 size_t logprobs_scratch_bytes(const LogprobsArgs& a);
 hipError_t launch_logprobs(const LogprobsArgs& a, void* scratch, hipStream_t s);

@@ -87,16 +87,19 @@ __global__ __launch_bounds__(256) void logprobs_any_kernel(const LogprobsArgs p)
   }
 }
 
-// ---- the usual path: one pass over the logits by independent waves, then one workgroup per row that joins them
+// ---- the usual path: one pass over the logits by independent waves, then one workgroup per row that joins them (rows of
+// up to four segments: both in one launch)
 //
 // A wave takes a segment of a row, GROUPS loads of 16 bytes per lane, keeps it in registers and leaves the segment's
 // maximum, sum and weighted sum, and the maximum of each neighbourhood (two loads of the wave: 512 f32 or 1024 f16
 // logits that lie side by side). The best top_k logits lie in the top_k neighbourhoods with the largest maxima (ties:
-// the lower one), so the joining workgroup looks at those again and at nothing else. Bound by the one read of the logits.
+// the lower one), so the joining workgroup looks at those again and at nothing else. Bound by the one read of the logits
+// where there are many rows, by the chain of dependent steps behind it where there are few.
 constexpr int GROUPS = 8;
 constexpr int HOODS = GROUPS / 2;          // neighbourhoods of a segment
-constexpr uint32_t MAX_HOODS = 4096;       // of a row: the joining workgroup keeps 16 per thread
-constexpr uint32_t MAX_CANDIDATES = 1024;  // logits that it ranks at once
+constexpr uint32_t MAX_HOODS = 4096;       // of a row
+constexpr uint32_t MAX_SEGMENTS = MAX_HOODS / HOODS;
+constexpr uint32_t MAX_CANDIDATES = 1024;  // logits that are ranked at once
 
 template <class T>
 constexpr uint32_t per_load = 16 / sizeof(T);
@@ -105,9 +108,10 @@ constexpr uint32_t hood_size = 2 * 64 * per_load<T>;
 template <class T>
 constexpr uint32_t segment_size = GROUPS * 64 * per_load<T>;
 
+// What a segment leaves: its maximum, the sums of e = 2^d and of e*d with d = (x - maximum) * c, and the maxima of its
+// neighbourhoods.
 struct SegmentStats {
-  float top, total, weighted;  // maximum of the logits; sum of e = 2^d; sum of e*d, d = (x - top) * c
-  float hood[HOODS];
+  float top, total, weighted, hood[HOODS];
 };
 
 // Elements of a row are numbered from the 16-byte boundary at or before its first one, so that every load is aligned.
@@ -115,19 +119,17 @@ template <class T>
 __device__ __forceinline__ uint32_t lead_of(const T* row) {
   return (uint32_t)(reinterpret_cast<uint64_t>(row) & 15u) / sizeof(T);
 }
-// per_load<T> logits from place `at` (a multiple of per_load); places outside the row read as `outside`
+// per_load<T> logits from place `at` (a multiple of per_load); places outside the row read as -inf
 template <class T>
-__device__ __forceinline__ void load_group(const T* row, uint32_t lead, uint32_t vocab, uint32_t at, float outside, float* x) {
+using Group = T __attribute__((ext_vector_type(16 / sizeof(T))));
+template <class T>
+__device__ __forceinline__ Group<T> load_group(const T* row, uint32_t lead, uint32_t vocab, uint32_t at) {
   constexpr uint32_t N = per_load<T>;
-  if (at >= lead && at + N <= lead + vocab) {
-    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
-    const vec v = *reinterpret_cast<const vec*>(row + (at - lead));
+  if (at >= lead && at + N <= lead + vocab) return *reinterpret_cast<const Group<T>*>(row + (at - lead));
+  Group<T> v;
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++) x[i] = (float)v[i];
-  } else {
-#pragma unroll
-    for (uint32_t i = 0; i < N; i++) x[i] = at + i >= lead && at + i < lead + vocab ? (float)row[at + i - lead] : outside;
-  }
+  for (uint32_t i = 0; i < N; i++) v[i] = at + i >= lead && at + i < lead + vocab ? row[at + i - lead] : (T)-INFINITY;
+  return v;
 }
 
 __device__ __forceinline__ float max_of_wave(float v) {
@@ -138,19 +140,21 @@ __device__ __forceinline__ float sum_of_wave(float v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
+// value and id of a candidate as one number: larger is better, ties to the lower id
+__device__ __forceinline__ unsigned long long rank_key(float v, uint32_t id) { return (unsigned long long)order_of(v) << 32 | (uint32_t)~id; }
+// the logit that has this place in the order
+__device__ __forceinline__ float value_of(uint32_t order) {
+  return order ? __builtin_bit_cast(float, order & 0x80000000u ? order & 0x7FFFFFFFu : ~order) : NAN;
+}
 
+// One wave reads one segment.
 template <class T>
-__global__ __launch_bounds__(256) void logits_segments_kernel(const LogprobsArgs p, SegmentStats* stats, uint32_t segments, float c) {
+__device__ __forceinline__ SegmentStats read_segment(const T* row, uint32_t lead, uint32_t vocab, uint32_t seg, float c) {
   constexpr uint32_t N = per_load<T>;
-  const uint32_t lane = threadIdx.x & 63u;
-  const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
-  const uint32_t r = (uint32_t)(unit / segments), seg = (uint32_t)(unit - (uint64_t)r * segments);
-  if (r >= p.rows) return;  // whole waves leave together
-  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
-  const uint32_t lead = lead_of(row), first = seg * segment_size<T>;
-  float x[GROUPS][N];
+  const uint32_t lane = threadIdx.x & 63u, first = seg * segment_size<T>;
+  Group<T> x[GROUPS];
 #pragma unroll
-  for (int g = 0; g < GROUPS; g++) load_group(row, lead, p.vocab, first + (g * 64 + lane) * N, -INFINITY, x[g]);
+  for (int g = 0; g < GROUPS; g++) x[g] = load_group(row, lead, vocab, first + (g * 64 + lane) * N);
   SegmentStats s;
   s.top = -INFINITY;
 #pragma unroll
@@ -159,61 +163,67 @@ __global__ __launch_bounds__(256) void logits_segments_kernel(const LogprobsArgs
 #pragma unroll
     for (int g = 2 * n; g < 2 * n + 2; g++)
 #pragma unroll
-      for (uint32_t i = 0; i < N; i++) m = fmaxf(m, x[g][i]);
+      for (uint32_t i = 0; i < N; i++) m = fmaxf(m, (float)x[g][i]);
     s.hood[n] = max_of_wave(m);
     s.top = fmaxf(s.top, s.hood[n]);
   }
-  const float top = s.top == -INFINITY ? 0.f : s.top;
+  const float from = s.top == -INFINITY ? 0.f : s.top;
   s.total = s.weighted = 0.f;
 #pragma unroll
   for (int g = 0; g < GROUPS; g++)
 #pragma unroll
     for (uint32_t i = 0; i < N; i++) {
-      const float d = (x[g][i] - top) * c, e = __builtin_amdgcn_exp2f(d);  // the difference first: exact or nearly so
+      const float d = ((float)x[g][i] - from) * c, e = __builtin_amdgcn_exp2f(d);  // the difference first: exact or nearly so
       s.total += e;
       s.weighted = __builtin_fmaf(e, fmaxf(d, -1e4f), s.weighted);  // e is 0 there; keeps 0 * -inf out of the sum
     }
   s.total = sum_of_wave(s.total);
   s.weighted = sum_of_wave(s.weighted);
-  if (lane == 0) stats[unit] = s;
+  return s;
 }
 
-// value and id of a candidate as one number: larger is better, ties to the lower id
-__device__ __forceinline__ unsigned long long rank_key(float v, uint32_t id) { return (unsigned long long)order_of(v) << 32 | (uint32_t)~id; }
-
-// the logit that has this place in the order
-__device__ __forceinline__ float value_of(uint32_t order) {
-  return order ? __builtin_bit_cast(float, order & 0x80000000u ? order & 0x7FFFFFFFu : ~order) : NAN;
+template <class T>
+__global__ __launch_bounds__(256) void logits_segments_kernel(const LogprobsArgs p, SegmentStats* stats, uint32_t segments, float c) {
+  const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6);
+  const uint32_t r = (uint32_t)(unit / segments), seg = (uint32_t)(unit - (uint64_t)r * segments);
+  if (r >= p.rows) return;  // whole waves leave together
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
+  const SegmentStats s = read_segment(row, lead_of(row), p.vocab, seg, c);
+  if ((threadIdx.x & 63u) == 0) stats[unit] = s;
 }
 
-// One workgroup of NT threads per row. A chain of dependent steps bounds it (statistics, their joint maximum, the bound,
-// the neighbourhoods, the places), so everything that does not depend on an earlier step is fetched first, and the
-// neighbourhoods are looked at by all waves at once.
-template <class T, int NT>
-__global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p, const SegmentStats* all, uint32_t segments, float c) {
+// The answer for row r from its segments' statistics, by a workgroup of NT threads. A chain of dependent steps bounds it
+// (statistics, their joint maximum, the bound, the neighbourhoods, the places), so what does not wait for anything is
+// fetched first, and all waves look at the neighbourhoods at once.
+template <class T, int NT, uint32_t MOST>
+__device__ __forceinline__ void answer_row(const LogprobsArgs& p, uint32_t r, const SegmentStats* stats, uint32_t segments, float c) {
   constexpr uint32_t N = per_load<T>, WAVES = NT / 64;
   __shared__ float red[3][WAVES];
   __shared__ __align__(16) uint32_t most[256];
+  __shared__ uint32_t above[256];
   __shared__ unsigned long long candidates[MAX_CANDIDATES], best[WAVES];
-  __shared__ uint16_t chosen[MAX_HOODS];
+  __shared__ uint16_t chosen[MOST * HOODS];
   __shared__ uint32_t count, chosen_count, bound;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r = blockIdx.x;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.row_stride;
   const uint32_t lead = lead_of(row);
-  const SegmentStats* stats = all + (uint64_t)r * segments;
+  int32_t token = -1;
+  if (tid == 0 && p.logprob) token = p.tokens[r];
+  const bool in_vocab = token >= 0 && (uint32_t)token < p.vocab;
+  float given = 0.f;
+  SegmentStats first;
+  first.top = -INFINITY;
+  if (tid < segments) first = stats[tid];
+  if (tid < 256u) above[tid] = 0;
+  if (tid == 0) count = chosen_count = bound = 0;
+
+  // ---- the sums, and the largest logit of each of 256 parts of the row
   const uint32_t K = p.top_ids || p.top_logprobs ? p.top_k : 0;
   const uint32_t hoods = (lead + p.vocab + hood_size<T> - 1) / hood_size<T>;
   const bool by_hood = hoods >= K;
   auto hood_order = [&](uint32_t n) { return order_of(stats[n / HOODS].hood[n % HOODS]); };
-  // what does not wait for anything
-  int32_t token = -1;
-  if (tid == 0 && p.logprob) token = p.tokens[r];
-  SegmentStats first;
-  first.top = -INFINITY;
-  first.total = first.weighted = 0.f;
-  if (tid < segments) first = stats[tid];
-  uint32_t mine = 0;  // the largest of this part of the row, 256 parts
   if (K && tid < 256u) {
+    uint32_t mine = 0;
     if (by_hood) {
       for (uint32_t n = tid; n < hoods; n += 256u) mine = max(mine, hood_order(n));
     } else {
@@ -221,12 +231,7 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
     }
     most[tid] = mine;
   }
-  float given = 0.f;
-  const bool in_vocab = token >= 0 && (uint32_t)token < p.vocab;
   if (in_vocab) given = (float)row[token];
-  if (tid == 0) count = chosen_count = bound = 0;
-
-  // ---- the sums
   float top = first.top;
   for (uint32_t s = tid + NT; s < segments; s += NT) top = fmaxf(top, stats[s].top);
   top = max_of_wave(top);
@@ -253,32 +258,34 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
     red[1][wave] = total;
     red[2][wave] = weighted;
   }
-  // ---- meanwhile a bound: the K-th largest of the 256 maxima; at least K logits reach it
-  if (K && tid < 256u) {
-    uint32_t above = 0;  // parts that come before this one
+  // ---- a bound: the K-th largest of those maxima; at least K logits reach it. A thread compares one part with 64 or 256.
+  if (K) {
+    const uint32_t mine = most[tid & 255u], own = (tid & 255u) >> 6;
+    uint32_t before = 0;  // parts that come before this one; an equal maximum of a lower part does
 #pragma unroll 1
-    for (uint32_t w = 0; w < 4; w++) {
-      const uint32_t limit = w < wave ? mine - 1u : mine;  // an equal maximum of a lower part comes first
-      if (w != wave) {
-#pragma unroll 4
+    for (uint32_t w = NT == 1024 ? tid >> 8 : 0; w < (NT == 1024 ? (tid >> 8) + 1 : 4); w++) {
+      const uint32_t limit = w < own ? mine - 1u : mine;
+      if (w != own) {
+#pragma unroll 8
         for (uint32_t j = 64 * w; j < 64 * w + 64; j += 4) {
           const u32x4 v = *reinterpret_cast<const u32x4*>(&most[j]);
-          above += (v.x > limit) + (v.y > limit) + (v.z > limit) + (v.w > limit);
+          before += (v.x > limit) + (v.y > limit) + (v.z > limit) + (v.w > limit);
         }
       } else {
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t j = 0; j < 64; j += 4) {
           const u32x4 v = *reinterpret_cast<const u32x4*>(&most[64 * w + j]);
-          above += v.x > mine || (v.x == mine && j < lane);
-          above += v.y > mine || (v.y == mine && j + 1 < lane);
-          above += v.z > mine || (v.z == mine && j + 2 < lane);
-          above += v.w > mine || (v.w == mine && j + 3 < lane);
+          before += v.x > mine || (v.x == mine && j < lane);
+          before += v.y > mine || (v.y == mine && j + 1 < lane);
+          before += v.z > mine || (v.z == mine && j + 2 < lane);
+          before += v.w > mine || (v.w == mine && j + 3 < lane);
         }
       }
     }
-    if (mine && above == K - 1) bound = mine;
+    atomicAdd(&above[tid & 255u], before);
   }
   __syncthreads();
+  if (K && tid < 256u && most[tid] && above[tid] == K - 1) bound = most[tid];
   total = weighted = 0.f;
 #pragma unroll
   for (uint32_t w = 0; w < WAVES; w++) {
@@ -294,6 +301,7 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
     if (p.entropy) p.entropy[r] = nothing ? 0.f : log_total - weighted / total * LN2;
   }
   if (!K) return;
+  __syncthreads();
   auto answer = [&](uint32_t place, unsigned long long key) {
     if (p.top_ids) p.top_ids[(size_t)r * K + place] = ~(uint32_t)key;
     if (p.top_logprobs) p.top_logprobs[(size_t)r * K + place] = logp(value_of((uint32_t)(key >> 32)));
@@ -311,15 +319,15 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
     if (by_hood) {
       for (uint32_t k = wave; k < chosen_count; k += WAVES) {
         const uint32_t from = (uint32_t)chosen[k] * hood_size<T>;
-        float x[2][N];
+        Group<T> x[2];
 #pragma unroll
-        for (uint32_t g = 0; g < 2; g++) load_group(row, lead, p.vocab, from + (g * 64 + lane) * N, 0.f, x[g]);
+        for (uint32_t g = 0; g < 2; g++) x[g] = load_group(row, lead, p.vocab, from + (g * 64 + lane) * N);
 #pragma unroll
         for (uint32_t g = 0; g < 2; g++) {
           const uint32_t at = from + (g * 64 + lane) * N;
 #pragma unroll
           for (uint32_t i = 0; i < N; i++)
-            if (at + i >= lead && at + i < lead + p.vocab) f(x[g][i], at + i - lead);
+            if (at + i >= lead && at + i < lead + p.vocab) f((float)x[g][i], at + i - lead);
         }
       }
     } else {
@@ -339,6 +347,7 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
     for (uint32_t i = tid; i < n; i += NT) {
       const unsigned long long key = candidates[i];
       uint32_t place = 0;
+#pragma unroll 8
       for (uint32_t j = 0; j < n; j++) place += candidates[j] > key;
       if (place < K) answer(place, key);
     }
@@ -403,24 +412,43 @@ __global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p,
   }
 }
 
-// Segments of a row, whatever its alignment.
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void logits_answer_kernel(const LogprobsArgs p, const SegmentStats* stats, uint32_t segments, float c) {
+  answer_row<T, NT, MAX_SEGMENTS>(p, blockIdx.x, stats + (uint64_t)blockIdx.x * segments, segments, c);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void logits_row_kernel(const LogprobsArgs p, uint32_t segments, float c) {
+  __shared__ SegmentStats stats[4];
+  const uint32_t seg = threadIdx.x >> 6;
+  if (seg < segments) {
+    const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)blockIdx.x * p.row_stride;
+    const SegmentStats s = read_segment(row, lead_of(row), p.vocab, seg, c);
+    if ((threadIdx.x & 63u) == 0) stats[seg] = s;
+  }
+  __syncthreads();
+  answer_row<T, 256, 4>(p, blockIdx.x, stats, segments, c);
+}
+
+// Segments of a row, whatever its alignment; 0: too long for the table of neighbourhoods.
 template <class T>
 uint32_t segments_of(uint32_t vocab) {
+  if ((uint64_t)vocab + per_load<T> > (uint64_t)MAX_HOODS * hood_size<T>) return 0;
   return (uint32_t)(((uint64_t)vocab + per_load<T> - 1 + segment_size<T> - 1) / segment_size<T>);
 }
 template <class T>
-bool segmented(uint32_t vocab) {
-  return (uint64_t)vocab + per_load<T> <= (uint64_t)MAX_HOODS * hood_size<T>;
-}
-template <class T>
 hipError_t launch_typed(const LogprobsArgs& a, void* scratch, hipStream_t s) {
-  if (!segmented<T>(a.vocab)) {
+  const uint32_t segments = segments_of<T>(a.vocab);
+  const float c = a.inv_temperature * 1.4426950408889634f;
+  if (!segments) {
     hipLaunchKernelGGL(logprobs_any_kernel<T>, dim3(a.rows), dim3(256), 0, s, a);
     return hipGetLastError();
   }
+  if (segments <= 4) {
+    hipLaunchKernelGGL(logits_row_kernel<T>, dim3(a.rows), dim3(256), 0, s, a, segments, c);
+    return hipGetLastError();
+  }
   SegmentStats* stats = static_cast<SegmentStats*>(scratch);
-  const uint32_t segments = segments_of<T>(a.vocab);
-  const float c = a.inv_temperature * 1.4426950408889634f;
   const uint64_t waves = (uint64_t)a.rows * segments;
   hipLaunchKernelGGL(logits_segments_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, a, stats, segments, c);
   // few rows: as many waves as a row can use; many: as many rows as fit
@@ -432,8 +460,8 @@ hipError_t launch_typed(const LogprobsArgs& a, void* scratch, hipStream_t s) {
 }  // namespace
 
 size_t logprobs_scratch_bytes(const LogprobsArgs& a) {
-  const bool takes = a.f16 ? segmented<_Float16>(a.vocab) : segmented<float>(a.vocab);
-  return takes ? (size_t)a.rows * (a.f16 ? segments_of<_Float16>(a.vocab) : segments_of<float>(a.vocab)) * sizeof(SegmentStats) : 0;
+  const uint32_t segments = a.f16 ? segments_of<_Float16>(a.vocab) : segments_of<float>(a.vocab);
+  return segments > 4 ? (size_t)a.rows * segments * sizeof(SegmentStats) : 0;
 }
 
 hipError_t launch_logprobs(const LogprobsArgs& a, void* scratch, hipStream_t s) {

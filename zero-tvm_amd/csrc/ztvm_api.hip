@@ -421,8 +421,8 @@ int ztvm_create(int device, ztvm_ctx** out) {
   }
   c->scratch = std::make_shared<DevicePool>(DeviceAlloc{device});
   if (!c->scratch->reserve(4u << 20)) return fail(nullptr, ZTVM_E_HIP, "ztvm_create: no device memory for the scratch buffer");
-  HIP_TRY(nullptr, hipMalloc(reinterpret_cast<void**>(&c->gemm_counters), (ZTVM_GEMM_SPLIT_TILES + ZTVM_ATTENTION_ARRIVALS) * sizeof(uint32_t)));
-  HIP_TRY(nullptr, hipMemset(c->gemm_counters, 0, (ZTVM_GEMM_SPLIT_TILES + ZTVM_ATTENTION_ARRIVALS) * sizeof(uint32_t)));
+  HIP_TRY(nullptr, hipMalloc(reinterpret_cast<void**>(&c->gemm_counters), (ZTVM_GEMM_SPLIT_TILES + ZTVM_ARRIVALS) * sizeof(uint32_t)));
+  HIP_TRY(nullptr, hipMemset(c->gemm_counters, 0, (ZTVM_GEMM_SPLIT_TILES + ZTVM_ARRIVALS) * sizeof(uint32_t)));
   HIP_TRY(nullptr, hipDeviceSynchronize());  // the fill runs on the null stream, which the context's stream does not wait for
   g.c = nullptr;
   *out = c;
