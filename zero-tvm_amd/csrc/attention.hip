@@ -839,7 +839,9 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
   }
 }
 
-// Adds the partial results of a row's splits, in their order. One wave per query row and head.
+// Adds the partial results of a row's splits, in their order. One wave per query row and head. BATCH: splits that a lane asks
+// for at once (few splits: the instructions of an empty batch are what the launch would wait for).
+template <uint32_t BATCH>
 __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t tile_rows, float lift) {
   const AttentionArgs& a = p.a;
   const KvView& c = a.cache;
@@ -861,9 +863,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
   const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits;
   const float* acc = p.partial + at * c.head_dim;
   const float2* ml = p.partial_ml + at;
-  // a lane takes four dims of every `ways`-th split; eight of them are asked for before the weights are known
+  // a lane takes four dims of every `ways`-th split; the first are asked for before the weights are known
   const uint32_t quads = c.head_dim / 4, ways = 64u / quads, way = lane / quads, d = (lane - way * quads) * 4;
-  constexpr uint32_t BATCH = 8;
   f4 x[BATCH];
   auto batch = [&](uint32_t s1) {
 #pragma unroll
@@ -974,7 +975,8 @@ hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.splits == 1 || KW > 1) return e;
   const uint32_t units = std::min(p.a.max_query, p.a.tokens) * p.a.heads;
-  hipLaunchKernelGGL(attention_join_kernel, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
+  auto join = g.splits * KD <= 16 ? attention_join_kernel<2> : attention_join_kernel<8>;
+  hipLaunchKernelGGL(join, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
   return hipGetLastError();
 }
 template <int KD, bool INT8>
