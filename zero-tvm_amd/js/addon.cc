@@ -4,6 +4,7 @@
 // Every failure becomes a JS exception carrying ztvm_last_error().
 #include <node_api.h>
 
+#include <cstddef>
 #include <cstdint>
 #include <cstring>
 #include <string>
@@ -586,6 +587,135 @@ napi_value KvQuantizeInt8(napi_env env, napi_callback_info info) {
   return rc ? throw_ztvm(env, (ztvm_ctx*)p, rc, "ztvm_kv_quantize_int8") : undefined(env);
 }
 
+// Descriptors of the verification dispatches: JS objects whose keys are the C field names, `cache` a nested one. Absent
+// fields stay zero; what a descriptor may hold is the library's to say.
+struct Field {
+  const char* name;
+  char kind;  // 'u' uint32, 'a' uint64, 'f' float
+  size_t offset;
+};
+bool read_fields(napi_env env, napi_value obj, const Field* fields, size_t n, void* to) {
+  napi_valuetype type;
+  if (napi_typeof(env, obj, &type) != napi_ok || type != napi_object) {
+    napi_throw_type_error(env, nullptr, "ztvm addon: expected a descriptor object");
+    return false;
+  }
+  for (size_t i = 0; i < n; i++) {
+    const Field& f = fields[i];
+    char* at = static_cast<char*>(to) + f.offset;
+    napi_value v;
+    bool has = false;
+    napi_has_named_property(env, obj, f.name, &has);
+    if (!has) continue;
+    napi_get_named_property(env, obj, f.name, &v);
+    double number = 0;
+    bool ok = true;
+    if (f.kind == 'u') ok = napi_get_value_uint32(env, v, reinterpret_cast<uint32_t*>(at)) == napi_ok;
+    else if (f.kind == 'f') ok = napi_get_value_double(env, v, &number) == napi_ok;
+    else if (!get_u64(env, v, reinterpret_cast<uint64_t*>(at))) return false;
+    if (!ok) {
+      napi_throw_type_error(env, nullptr, (std::string("ztvm addon: descriptor field '") + f.name + "' must be a number").c_str());
+      return false;
+    }
+    if (f.kind == 'f') *reinterpret_cast<float*>(at) = static_cast<float>(number);
+  }
+  return true;
+}
+#define U(T, name) {#name, 'u', offsetof(T, name)}
+#define A(T, name) {#name, 'a', offsetof(T, name)}
+#define F(T, name) {#name, 'f', offsetof(T, name)}
+const Field kCacheFields[] = {
+    U(ztvm_kv_cache, format), U(ztvm_kv_cache, kv_heads), U(ztvm_kv_cache, head_dim), U(ztvm_kv_cache, page_size),
+    U(ztvm_kv_cache, kv_page_stride), U(ztvm_kv_cache, head_page_stride), U(ztvm_kv_cache, v_page_offset), U(ztvm_kv_cache, pages_offset),
+    U(ztvm_kv_cache, scales_offset), A(ztvm_kv_cache, pages_capacity), A(ztvm_kv_cache, scales_capacity), A(ztvm_kv_cache, pages),
+    A(ztvm_kv_cache, scales)};
+const Field kRopeFields[] = {
+    U(ztvm_rope_append_desc, tokens), U(ztvm_rope_append_desc, heads), U(ztvm_rope_append_desc, rotary_dim), U(ztvm_rope_append_desc, interleaved),
+    U(ztvm_rope_append_desc, qkv_stride), U(ztvm_rope_append_desc, q_stride), F(ztvm_rope_append_desc, attn_factor), A(ztvm_rope_append_desc, qkv),
+    A(ztvm_rope_append_desc, q_out), A(ztvm_rope_append_desc, frequencies), A(ztvm_rope_append_desc, positions), A(ztvm_rope_append_desc, slots)};
+const Field kReadFields[] = {U(ztvm_kv_read_desc, tokens), U(ztvm_kv_read_desc, out_stride), A(ztvm_kv_read_desc, k_out), A(ztvm_kv_read_desc, v_out),
+                             A(ztvm_kv_read_desc, slots)};
+const Field kAttentionFields[] = {
+    U(ztvm_attention_desc, tokens), U(ztvm_attention_desc, sequences), U(ztvm_attention_desc, heads), U(ztvm_attention_desc, max_query),
+    U(ztvm_attention_desc, max_kv), U(ztvm_attention_desc, q_stride), U(ztvm_attention_desc, out_stride), U(ztvm_attention_desc, page_table_stride),
+    U(ztvm_attention_desc, mask_words), F(ztvm_attention_desc, scale), A(ztvm_attention_desc, q), A(ztvm_attention_desc, out),
+    A(ztvm_attention_desc, lse), A(ztvm_attention_desc, query_start), A(ztvm_attention_desc, kv_length), A(ztvm_attention_desc, page_table),
+    A(ztvm_attention_desc, tree_mask)};
+const Field kLogprobsFields[] = {
+    U(ztvm_token_logprobs_desc, rows), U(ztvm_token_logprobs_desc, vocab), U(ztvm_token_logprobs_desc, row_stride),
+    U(ztvm_token_logprobs_desc, logits_f16), U(ztvm_token_logprobs_desc, top_k), F(ztvm_token_logprobs_desc, inv_temperature),
+    A(ztvm_token_logprobs_desc, logits), A(ztvm_token_logprobs_desc, tokens), A(ztvm_token_logprobs_desc, logprob),
+    A(ztvm_token_logprobs_desc, entropy), A(ztvm_token_logprobs_desc, top_ids), A(ztvm_token_logprobs_desc, top_logprobs)};
+#undef U
+#undef A
+#undef F
+
+// (ctx, desc). A null ctx is passed on: the library checks the descriptor before it looks at the context.
+template <class Desc, size_t N>
+napi_value call_desc(napi_env env, napi_callback_info info, const Field (&fields)[N], ztvm_kv_cache Desc::*cache, int (*fn)(ztvm_ctx*, const Desc*),
+                     const char* what) {
+  napi_value a[2];
+  if (!get_args(env, info, 2, a)) return nullptr;
+  void* p = nullptr;
+  napi_valuetype type;
+  napi_typeof(env, a[0], &type);
+  if (type != napi_null && !get_ptr(env, a[0], &p)) return nullptr;
+  Desc d;
+  memset(&d, 0, sizeof d);
+  if (!read_fields(env, a[1], fields, N, &d)) return nullptr;
+  if (cache) {
+    napi_value c;
+    bool has = false;
+    napi_has_named_property(env, a[1], "cache", &has);
+    if (has) {
+      napi_get_named_property(env, a[1], "cache", &c);
+      if (!read_fields(env, c, kCacheFields, sizeof kCacheFields / sizeof kCacheFields[0], &(d.*cache))) return nullptr;
+    }
+  }
+  const int rc = fn(static_cast<ztvm_ctx*>(p), &d);
+  return rc ? throw_ztvm(env, static_cast<ztvm_ctx*>(p), rc, what) : undefined(env);
+}
+napi_value RopeAppend(napi_env env, napi_callback_info info) {
+  return call_desc<ztvm_rope_append_desc>(env, info, kRopeFields, &ztvm_rope_append_desc::cache, ztvm_rope_append, "ztvm_rope_append");
+}
+napi_value KvRead(napi_env env, napi_callback_info info) {
+  return call_desc<ztvm_kv_read_desc>(env, info, kReadFields, &ztvm_kv_read_desc::cache, ztvm_kv_read, "ztvm_kv_read");
+}
+napi_value Attention(napi_env env, napi_callback_info info) {
+  return call_desc<ztvm_attention_desc>(env, info, kAttentionFields, &ztvm_attention_desc::cache, ztvm_attention, "ztvm_attention");
+}
+napi_value TokenLogprobs(napi_env env, napi_callback_info info) {
+  return call_desc<ztvm_token_logprobs_desc>(env, info, kLogprobsFields, nullptr, ztvm_token_logprobs, "ztvm_token_logprobs");
+}
+
+// (kind, rotaryDim, theta, factor, original, low, high) -> { table: Float64Array, attnFactor }
+napi_value RopeFrequencies(napi_env env, napi_callback_info info) {
+  napi_value a[7];
+  if (!get_args(env, info, 7, a)) return nullptr;
+  uint32_t kind = 0, dim = 0;
+  double v[5];
+  bool ok = napi_get_value_uint32(env, a[0], &kind) == napi_ok && napi_get_value_uint32(env, a[1], &dim) == napi_ok;
+  for (int i = 0; i < 5; i++) ok = ok && napi_get_value_double(env, a[2 + i], &v[i]) == napi_ok;
+  if (!ok) {
+    napi_throw_type_error(env, nullptr, "ztvm addon: ropeFrequencies takes seven numbers");
+    return nullptr;
+  }
+  double table[256];  // the library refuses rotary_dim > 512
+  float factor = 0.f;
+  const int rc = ztvm_rope_frequencies(kind, dim, v[0], v[1], v[2], v[3], v[4], table, &factor);
+  if (rc) return throw_ztvm(env, nullptr, rc, "ztvm_rope_frequencies");
+  void* data = nullptr;
+  napi_value buffer, array, number, out;
+  NAPI_OK(env, napi_create_arraybuffer(env, dim / 2 * sizeof(double), &data, &buffer));
+  memcpy(data, table, dim / 2 * sizeof(double));
+  NAPI_OK(env, napi_create_typedarray(env, napi_float64_array, dim / 2, buffer, 0, &array));
+  NAPI_OK(env, napi_create_double(env, factor, &number));
+  NAPI_OK(env, napi_create_object(env, &out));
+  NAPI_OK(env, napi_set_named_property(env, out, "table", array));
+  NAPI_OK(env, napi_set_named_property(env, out, "attnFactor", number));
+  return out;
+}
+
 napi_value Init(napi_env env, napi_value exports) {
   struct E { const char* name; napi_callback fn; };
   static const E table[] = {
@@ -596,7 +726,8 @@ napi_value Init(napi_env env, napi_value exports) {
       {"siluMul", SiluMul}, {"moeCombine", MoeCombine}, {"moeRouterLogits", MoeRouterLogits}, {"moeRouterTopk", MoeRouterTopk},
       {"moeSlotTranslate", MoeSlotTranslate}, {"ffnGated", FfnGated}, {"ffnGatedPrologue", FfnGatedPrologue}, {"repackPart", RepackPart},
       {"repackPermuteRows", RepackPermuteRows}, {"repackDequantSplit", RepackDequantSplit}, {"qkvFused", QkvFused},
-      {"qkvFusedScratch", QkvFusedScratch}, {"kvQuantizeInt8", KvQuantizeInt8}};
+      {"qkvFusedScratch", QkvFusedScratch}, {"kvQuantizeInt8", KvQuantizeInt8}, {"ropeAppend", RopeAppend}, {"kvRead", KvRead},
+      {"attention", Attention}, {"tokenLogprobs", TokenLogprobs}, {"ropeFrequencies", RopeFrequencies}};
   for (const E& e : table) {
     napi_value fn;
     if (napi_create_function(env, e.name, NAPI_AUTO_LENGTH, e.fn, nullptr, &fn) != napi_ok) return nullptr;

@@ -17,6 +17,26 @@ export declare class Uniform { words: number[]; writeU32(byteOffset: number, val
 export interface ZtvmBuffer { readonly size: number; readonly label: string; readonly addr: bigint; destroy(): void }
 export type BindEntry = ZtvmBuffer | { buffer: ZtvmBuffer; offset: number; size: number } | Uniform
 export interface BindGroup { pipeline: Pipeline; pod: Uniform }
+export interface KvCacheDesc {
+  format: number; kv_heads: number; head_dim: number; page_size: number; kv_page_stride?: number; head_page_stride?: number
+  v_page_offset?: number; pages_offset?: number; scales_offset?: number; pages_capacity: bigint; scales_capacity?: bigint
+  pages: bigint; scales?: bigint
+}
+export type Bound = BindEntry | bigint
+export interface RopeAppendDesc {
+  tokens: number; heads: number; rotary_dim: number; interleaved?: 0 | 1; qkv_stride: number; q_stride: number; attn_factor: number
+  qkv: Bound; q_out: Bound; frequencies: Bound; positions: Bound; slots: Bound; cache: KvCacheDesc
+}
+export interface KvReadDesc { tokens: number; out_stride: number; k_out?: Bound; v_out?: Bound; slots: Bound; cache: KvCacheDesc }
+export interface AttentionDesc {
+  tokens: number; sequences: number; heads: number; max_query: number; max_kv: number; q_stride: number; out_stride: number
+  page_table_stride?: number; mask_words?: number; scale: number; q: Bound; out: Bound; lse?: Bound; query_start: Bound
+  kv_length: Bound; page_table?: Bound; tree_mask?: Bound; cache: KvCacheDesc
+}
+export interface TokenLogprobsDesc {
+  rows: number; vocab: number; row_stride: number; logits_f16?: 0 | 1; top_k?: number; inv_temperature: number; logits: Bound
+  tokens?: Bound; logprob?: Bound; entropy?: Bound; top_ids?: Bound; top_logprobs?: Bound
+}
 export declare class Device {
   constructor(index?: number)
   close(): void
@@ -47,6 +67,12 @@ export declare class Device {
     headDim: number; ropeTheta: number }): void
   kvQuantizeInt8(bufs: BindEntry[], pod: Uniform, model: { kvHeads: number; headDim: number; pageSize: number },
     tokens?: number): void
+  kvCache(c: { format: number; kvHeads: number; headDim: number; pageSize: number; pages: BindEntry; scales?: BindEntry
+    kvPageStride?: number; headPageStride?: number; vPageOffset?: number; pagesOffset?: number; scalesOffset?: number }): KvCacheDesc
+  ropeAppend(desc: RopeAppendDesc): void
+  kvRead(desc: KvReadDesc): void
+  attention(desc: AttentionDesc): void
+  tokenLogprobs(desc: TokenLogprobsDesc): void
   matmul(desc: MatmulDesc): void
   matmulStatic(desc: MatmulDesc): void
   readProbe(buffer: ZtvmBuffer, bytes: number, sink: ZtvmBuffer): void
@@ -58,6 +84,10 @@ export declare class Device {
   sync(): void
 }
 export declare const KERNEL: { AUTO: 0; GEMV: 1; SKINNY: 2; GEMM: 3; ROWS: 4 }
+export declare const KV: { F16: 0; INT8: 1 }
+export declare const ROPE: { PLAIN: 0; LINEAR: 1; PIECEWISE: 2; YARN: 3 }
+export declare function ropeFrequencies(kind: number, rotaryDim: number, theta: number,
+  opts?: { factor?: number; original?: number; low?: number; high?: number }): { table: Float64Array; attnFactor: number }
 export declare const INT4_MATMUL_VARIANTS: ReadonlyArray<Int4MatmulOpts>
 export declare const GEMM_ENTRIES: ReadonlyArray<string>
 export declare const INT8_ENTRIES: ReadonlyArray<string>

@@ -321,6 +321,37 @@ class Device {
       BigInt(Math.floor(bufs[2].size / 4)), BigInt(Math.floor(bufs[3].size / 2)),
       model.kvHeads, model.headDim, model.pageSize, tokens === undefined ? 1 : tokens, w[0], w[1], w[2])
   }
+  /**
+   * A paged cache for the verification dispatches: { format: KV.F16 | KV.INT8, kvHeads, headDim, pageSize, pages, scales }. The
+   * F16 strides default to the dense layout [page][K, V][head][slot][dim]; the capacities are the sizes of the bound buffers.
+   */
+  kvCache(c) {
+    const int8 = c.format === KV.INT8, hps = c.headPageStride || c.pageSize * c.headDim
+    const vpo = c.vPageOffset || c.kvHeads * hps, size = (b, unit) => (b ? BigInt(Math.floor(b.size / unit)) : 0n)
+    const out = {
+      format: c.format, kv_heads: c.kvHeads, head_dim: c.headDim, page_size: c.pageSize, pages_offset: c.pagesOffset || 0,
+      scales_offset: c.scalesOffset || 0, pages_capacity: size(c.pages, int8 ? 4 : 2), scales_capacity: size(c.scales, 2),
+      pages: this._a(c.pages), scales: this._a(c.scales),
+    }
+    if (!int8) Object.assign(out, { head_page_stride: hps, v_page_offset: vpo, kv_page_stride: c.kvPageStride || vpo + c.kvHeads * hps })
+    return out
+  }
+  // a descriptor whose buffer fields may be buffers, regions or addresses
+  _d(desc, fields) {
+    const out = Object.assign({}, desc)
+    for (const f of fields) if (out[f] !== undefined && typeof out[f] !== 'bigint') out[f] = this._a(out[f])
+    return out
+  }
+  /** rotary positions and the append of K and V for several tokens (fields of ztvm_rope_append_desc; cache from kvCache()) */
+  ropeAppend(desc) { addon().ropeAppend(this.ctx, this._d(desc, ['qkv', 'q_out', 'frequencies', 'positions', 'slots'])) }
+  /** rows of the cache read back as f16 (fields of ztvm_kv_read_desc) */
+  kvRead(desc) { addon().kvRead(this.ctx, this._d(desc, ['k_out', 'v_out', 'slots'])) }
+  /** attention over the paged cache: one token, chains, trees of drafted tokens (fields of ztvm_attention_desc) */
+  attention(desc) { addon().attention(this.ctx, this._d(desc, ['q', 'out', 'lse', 'query_start', 'kv_length', 'page_table', 'tree_mask'])) }
+  /** log probabilities of given tokens, entropy, best alternatives (fields of ztvm_token_logprobs_desc) */
+  tokenLogprobs(desc) {
+    addon().tokenLogprobs(this.ctx, this._d(desc, ['logits', 'tokens', 'logprob', 'entropy', 'top_ids', 'top_logprobs']))
+  }
   beginEncoder() { addon().recordBegin(this.ctx) }
   finishEncoder() { return addon().recordEnd(this.ctx) }
   submit(cmdbuf) { addon().submit(this.ctx, cmdbuf) }
@@ -368,8 +399,15 @@ function moePods(dModel, ffn, slots, bits) {
   }
 }
 
+const KV = { F16: 0, INT8: 1 }
+const ROPE = { PLAIN: 0, LINEAR: 1, PIECEWISE: 2, YARN: 3 }
+/** The frequency table of ropeAppend: { table: Float64Array (to upload), attnFactor }. */
+function ropeFrequencies(kind, rotaryDim, theta, o = {}) {
+  return addon().ropeFrequencies(kind, rotaryDim, theta, o.factor === undefined ? 1 : o.factor, o.original || 0, o.low || 0, o.high || 0)
+}
+
 module.exports = {
-  KERNEL, Device, Uniform, int4MatmulEntry, checkOpts, INT4_MATMUL_VARIANTS, GEMM_ENTRIES, INT8_ENTRIES, ALL_ENTRIES, createPipeline,
+  KERNEL, KV, ROPE, ropeFrequencies, Device, Uniform, int4MatmulEntry, checkOpts, INT4_MATMUL_VARIANTS, GEMM_ENTRIES, INT8_ENTRIES, ALL_ENTRIES, createPipeline,
   resolveMatmul, resolveChunkCap, pickChunkGemm, foldGridX, densePod, moePods,
   // boot-time choice of the prefill GEMM by measurement (gemm_tune.js)
   TUNE_VERSION: tune.TUNE_VERSION, TUNE_TTL_MS: tune.TUNE_TTL_MS, TUNE_MS: tune.TUNE_MS, tuneKey: tune.tuneKey,
