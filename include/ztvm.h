@@ -405,8 +405,11 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  * sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
  * matter. Rows outside every sequence are left as they were.
  * max_query and max_kv bound n_b and kv_length[b] (the lengths are read on the device, so a recorded step can be
- * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen. Scratch
- * for the joined partial results comes from the context and depends on the descriptor only. */
+ * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen. The work is
+ * split over workgroups by these bounds, so bounds near the lengths are the fast ones. Scratch for the joined partial
+ * results comes from the context and depends on the descriptor only.
+ * Head sizes of 64, 96, 128 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
+ * cores; everything else is right as well, by a plain kernel. */
 typedef struct ztvm_attention_desc {
   uint32_t tokens;    /* rows of q, out, lse and tree_mask */
   uint32_t sequences, heads;
@@ -414,7 +417,7 @@ typedef struct ztvm_attention_desc {
   uint32_t q_stride, out_stride; /* f16 elements between token rows; head h starts at element h*head_dim */
   uint32_t page_table_stride;
   uint32_t mask_words; /* 64-bit words per token of tree_mask; at least max_query / 64, rounded up */
-  float scale;         /* finite */
+  float scale;         /* finite, at most 1e30 in magnitude */
   uint64_t q, out;
   uint64_t lse;         /* f32 [tokens][heads], or 0 */
   uint64_t query_start; /* i32 [sequences + 1], ascending */

@@ -353,6 +353,32 @@ def test_recorded_steps(ctx, capi):
             ctx.cmdbuf_destroy(cb)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_loose_bounds(ctx, capi, int8):
+    """Bounds far past what there is change neither results nor, in size, the scratch."""
+    s = Step(25, 8, 2, 128, 16, [(3, 200), (1, 60)], int8, tree="tree", mask_words=1)
+    s.table = np.concatenate([s.table, np.full((2, 4096), -1, np.int32)], 1)
+    s.check(ctx, capi, max_kv=65536)
+    s = Step(26, 8, 2, 128, 16, [(3, 200), (1, 60)], int8)
+    s.check(ctx, capi, max_query=(1 << 30) - 1)
+
+
+def test_two_contexts_at_once(ctx, capi):
+    """Two contexts on one GPU, their dispatches in flight together: scratch and counters are each one's own."""
+    a, b = Step(27, 8, 2, 128, 16, [(1, 4000), (1, 3000)]), Step(28, 8, 2, 128, 16, [(1, 2500), (1, 3999)])
+    other = capi.Context(0)
+    try:
+        with Dev(ctx) as da, Dev(other) as db:
+            x, y = a.desc(ctx, capi, da), b.desc(other, capi, db)
+            for _ in range(20):
+                ctx.attention(x)
+                other.attention(y)
+            a.compare(*a.got(ctx))
+            b.compare(*b.got(other))
+    finally:
+        other.close()
+
+
 def test_nothing_to_do(ctx, capi):
     s = Step(22, 4, 2, 64, 16, [(2, 20)])
     with Dev(ctx) as d:

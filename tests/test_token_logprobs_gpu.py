@@ -140,6 +140,18 @@ def test_extreme_scales(ctx, capi, scale):
     assert np.allclose(got["entropy"], entropy, atol=1e-4)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(np.float32, 2097148), (np.float32, 2097152), (np.float16, 4194300), (np.float16, 4200001)])
+def test_rows_at_and_past_the_table_of_neighbourhoods(ctx, capi, dtype, vocab):
+    x = (np.random.default_rng(10).standard_normal((2, vocab)) * 3).astype(dtype)
+    check(ctx, capi, x, [7, vocab - 1], 3)
+
+
+@pytest.mark.parametrize("rows", [513, 1500])
+def test_many_rows(ctx, capi, rows):
+    x = (np.random.default_rng(rows).standard_normal((rows, 9001)) * 3).astype(np.float16)
+    check(ctx, capi, x, np.arange(rows), 9)
+
+
 def test_offsets_past_32_bits(ctx, capi):
     """Rows whose elements lie past 2^32 of the array."""
     vocab, stride, rows = 2000, 1 << 31, 3

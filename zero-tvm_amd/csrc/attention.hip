@@ -923,8 +923,8 @@ bool mfma_takes(const AttentionArgs& a) {
   if (at % 16 || reinterpret_cast<uint64_t>(c.scales) % 4) return false;
   if ((reinterpret_cast<uint64_t>(a.q) | reinterpret_cast<uint64_t>(a.out)) & 15u || a.q_stride % 8 || a.out_stride % 8) return false;
   // the grid, and key positions a few turns past the last one, stay inside 31 bits
-  const uint64_t rows = (uint64_t)std::min(a.max_query, a.tokens) * a.heads;
-  return rows < (1u << 20) && a.max_kv < (1u << 30) && (uint64_t)a.sequences * c.kv_heads < (1u << 20);
+  const uint64_t rows = (uint64_t)a.max_query * (a.heads / c.kv_heads);
+  return rows <= 64ull * 65535u && a.max_query * (uint64_t)a.heads < (1ull << 31) && a.max_kv < (1u << 30) && (uint64_t)a.sequences * c.kv_heads < (1u << 20);
 }
 
 struct MfmaPlan {
@@ -932,18 +932,12 @@ struct MfmaPlan {
   uint32_t rows, row_tiles, splits, chunk;
   size_t partial_bytes, bytes;
 };
-#ifndef ATTN_LEAST
-#define ATTN_LEAST 2u
-#endif
-#ifndef ATTN_KW1
-#define ATTN_KW1 2
-#endif
 MfmaPlan mfma_plan(const AttentionArgs& a) {
   MfmaPlan g{};
   const uint32_t group = a.heads / a.cache.kv_heads;
-  const uint64_t rows = (uint64_t)std::min(a.max_query, a.tokens) * group;
+  const uint64_t rows = (uint64_t)a.max_query * group;
   const bool wide = a.cache.head_dim > 128;
-  if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = wide ? 2 : ATTN_KW1;
+  if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = 2;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
   else g.qt = rows <= 64 || wide ? 1 : 2, g.rw = 4, g.kw = 1;
   g.rows = 16 * g.qt * g.rw;
@@ -951,7 +945,7 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
   // enough workgroups for a few rounds of the CUs, none with less than four turns of its waves
   const uint64_t want = g.rw == 1 ? 2048 : a.sequences == 1 ? 512 : 1024;
-  const uint32_t unit = std::max(32u * g.kw, 64u), least = unit * (g.kw > 1 ? ATTN_LEAST : 4u);
+  const uint32_t unit = std::max(32u * g.kw, 64u), least = unit * (g.kw > 1 ? 2u : 4u);
   uint64_t splits = (want + groups - 1) / groups;
   splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, (a.max_kv + least - 1) / least, (uint64_t)MOST_SPLITS}));
   g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + unit - 1) / unit * unit);
@@ -974,7 +968,7 @@ hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t
   hipLaunchKernelGGL(kernel, grid, dim3(64 * RW * KW), Shape::LDS, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || g.splits == 1 || KW > 1) return e;
-  const uint32_t units = std::min(p.a.max_query, p.a.tokens) * p.a.heads;
+  const uint32_t units = p.a.max_query * p.a.heads;
   auto join = g.splits * KD <= 16 ? attention_join_kernel<2> : attention_join_kernel<8>;
   hipLaunchKernelGGL(join, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
   return hipGetLastError();
@@ -986,7 +980,7 @@ hipError_t launch_mfma_dim(const MfmaParams& p, const MfmaPlan& g, hipStream_t s
   if (g.rw == 4 && g.qt == 2) return launch_mfma_shape<KD, INT8, (KD > 4 ? 1 : 2), 4, 1, NS>(p, g, s);
   if (g.rw == 4) return launch_mfma_shape<KD, INT8, 1, 4, 1, NS>(p, g, s);
   if (g.qt == 2) return launch_mfma_shape<KD, INT8, 2, 1, KW, 1>(p, g, s);
-  return launch_mfma_shape<KD, INT8, 1, 1, (KD > 4 ? 2 : ATTN_KW1), 1>(p, g, s);
+  return launch_mfma_shape<KD, INT8, 1, 1, 2, 1>(p, g, s);
 }
 
 }  // namespace

@@ -929,7 +929,7 @@ int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
   const uint64_t width = (uint64_t)d->heads * d->cache.head_dim;
   if (d->q_stride < width || d->out_stride < width)
     return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: q_stride=%u or out_stride=%u is less than a row (%llu)", d->q_stride, d->out_stride, (unsigned long long)width);
-  if (!std::isfinite(d->scale)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: scale must be finite");
+  if (!(std::fabs(d->scale) <= 1e30f)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: scale must be finite, at most 1e30");
   if (!d->q || !d->out || !d->query_start || !d->kv_length) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: null buffer");
   if (((d->q | d->out) & 1u) || ((d->lse | d->query_start | d->kv_length | d->page_table) & 3u) || (d->tree_mask & 7u))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: misaligned buffer (q and out 2, lse, query_start, kv_length and page_table 4, tree_mask 8 bytes)");
@@ -954,7 +954,8 @@ int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
   a.kv_length = reinterpret_cast<const int32_t*>(d->kv_length);
   a.page_table = reinterpret_cast<const int32_t*>(d->page_table);
   a.tree_mask = reinterpret_cast<const uint64_t*>(d->tree_mask);
-  a.tokens = d->tokens; a.sequences = d->sequences; a.heads = d->heads; a.max_query = d->max_query; a.max_kv = d->max_kv;
+  a.tokens = d->tokens; a.sequences = d->sequences; a.heads = d->heads; a.max_kv = d->max_kv;
+  a.max_query = d->max_query < d->tokens ? d->max_query : d->tokens;  // no sequence has more rows than there are
   a.q_stride = d->q_stride; a.out_stride = d->out_stride; a.page_table_stride = d->page_table_stride; a.mask_words = d->mask_words;
   a.scale = d->scale;
   DeviceGuard g(ctx->device);
