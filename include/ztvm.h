@@ -354,7 +354,7 @@ typedef struct ztvm_kv_cache {
  * negative or in a page outside the cache stores nothing (its Q row is still written): that is how rows that only
  * pad a batch are marked. Two tokens of one call must not name the same slot. */
 typedef struct ztvm_rope_append_desc {
-  uint32_t tokens, heads;
+  uint32_t tokens, heads; /* tokens below 2^24 */
   uint32_t rotary_dim;  /* even, 2..head_dim */
   uint32_t interleaved; /* 0 | 1 */
   uint32_t qkv_stride, q_stride; /* f16 elements between token rows */
@@ -411,9 +411,9 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  * Head sizes of 64, 96, 128 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
  * cores; everything else is right as well, by a plain kernel. */
 typedef struct ztvm_attention_desc {
-  uint32_t tokens;    /* rows of q, out, lse and tree_mask */
+  uint32_t tokens;    /* rows of q, out, lse and tree_mask; below 2^24 */
   uint32_t sequences, heads;
-  uint32_t max_query, max_kv;
+  uint32_t max_query, max_kv;    /* each below 2^30 */
   uint32_t q_stride, out_stride; /* f16 elements between token rows; head h starts at element h*head_dim */
   uint32_t page_table_stride;
   uint32_t mask_words; /* 64-bit words per token of tree_mask; at least max_query / 64, rounded up */
@@ -436,7 +436,7 @@ ZTVM_API int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* desc);
  * has log probabilities -inf and entropy 0. A NaN or +inf among the logits makes the row's log probabilities and
  * entropy NaN; the ids still follow the order of the logits, NaN last. */
 typedef struct ztvm_token_logprobs_desc {
-  uint32_t rows, vocab;
+  uint32_t rows, vocab;   /* below 2^24 and 2^31 */
   uint32_t row_stride;    /* elements between rows of logits, >= vocab */
   uint32_t logits_f16;    /* 0: f32 logits (out_f32 of the LM head), 1: f16 */
   uint32_t top_k;         /* 0..min(vocab, 64) */

@@ -363,6 +363,70 @@ def test_loose_bounds(ctx, capi, int8):
     s.check(ctx, capi, max_query=(1 << 30) - 1)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (16, 1, 64), (4, 1, 256), (3, 3, 20)])
+def test_more_queries_than_keys(ctx, capi, heads, kv_heads, dim, int8):
+    """The first tokens of such a sequence see nothing, over several row tiles."""
+    Step(29, heads, kv_heads, dim, 16, [(100, 30), (70, 70), (40, 0), (5, 300)], int8).check(ctx, capi)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("queries", [1, 5, 12, 40])
+@pytest.mark.parametrize("page", [32, 48, 256, 1024])
+def test_page_sizes(ctx, capi, page, queries, int8):
+    Step(page + queries, 8, 2, 128, page, [(queries, 700), (queries, 1025), (queries, 48)], int8, tree="tree").check(ctx, capi)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("queries", [1, 5, 12, 40])
+def test_negative_and_zero_scales(ctx, capi, queries, int8):
+    s = Step(30, 8, 2, 128, 16, [(queries, 700), (queries, 130)], int8)
+    for scale in (-0.125, 0.0):
+        s.scale = scale
+        s.check(ctx, capi)
+
+
+@pytest.mark.parametrize("dim", [128, 20])
+@pytest.mark.parametrize("bound", [1, 7, 30])
+def test_queries_past_the_bound_stay(ctx, capi, bound, dim):
+    s = Step(31, 8, 2, dim, 16, [(40, 200), (3, 90)])
+    with Dev(ctx) as d:
+        ctx.attention(s.desc(ctx, capi, d, max_query=bound))
+        out, lse = s.got(ctx)
+    width = s.heads * s.dim
+    written = np.array([t - s.starts[b] < bound for b in range(2) for t in range(s.starts[b], s.starts[b + 1])])
+    assert np.all(out[~written] == 7.0) and np.all(lse[~written] == 7.0)
+    want, want_lse, *rest = s.want()
+    ref.close_attention(out[written].reshape(-1, s.heads, s.dim), lse[written], want[written], want_lse[written], *[r[written] for r in rest], s.dim, 200)
+
+
+def test_recordings_that_share_the_scratch(ctx, capi):
+    """Two recorded steps of one context, replayed in turn with eager calls between them."""
+    a, b = Step(32, 8, 2, 128, 16, [(1, 4000), (1, 3000)]), Step(33, 8, 2, 128, 16, [(40, 2500), (12, 3999)], True, tree="tree")
+    c = Step(34, 16, 2, 64, 16, [(4, 5000)])
+    with Dev(ctx) as da, Dev(ctx) as db, Dev(ctx) as dc:
+        x, y, z = a.desc(ctx, capi, da), b.desc(ctx, capi, db), c.desc(ctx, capi, dc)
+        recorded = []
+        for step in (x, y):
+            ctx.attention(step)                              # the scratch grows outside the recording
+            ctx.record_begin()
+            ctx.attention(step)
+            recorded.append(ctx.record_end())
+        for _ in range(4):
+            for step in (a, b, c):
+                ctx.upload(step.out, np.full(step.out_bytes // 2, 7.0, np.float16))
+                ctx.upload(step.lse, np.full(step.lse_bytes // 4, 7.0, np.float32))
+            ctx.submit(recorded[0])
+            ctx.submit(recorded[1])
+            ctx.attention(z)
+            ctx.submit(recorded[0])
+            ctx.sync()
+            for step in (a, b, c):
+                step.compare(*step.got(ctx))
+        for r in recorded:
+            ctx.cmdbuf_destroy(r)
+
+
 def test_two_contexts_at_once(ctx, capi):
     """Two contexts on one GPU, their dispatches in flight together: scratch and counters are each one's own."""
     a, b = Step(27, 8, 2, 128, 16, [(1, 4000), (1, 3000)]), Step(28, 8, 2, 128, 16, [(1, 2500), (1, 3999)])

@@ -165,3 +165,17 @@ def test_frequencies(capi):
 def test_frequencies_refuse(capi, args, needle):
     with pytest.raises(capi.ZtvmError, match=needle):
         capi.rope_frequencies(*args)
+
+
+def test_limits_of_a_launch(capi):
+    """The largest counts a launch takes, and one more."""
+    rope = dict(tokens=(1 << 24) - 1, heads=4, rotary_dim=64, qkv_stride=512, q_stride=256, attn_factor=1.0, qkv=0x100000, q_out=1 << 45,
+                frequencies=0x3000, positions=0x4000, slots=0x5000, cache=f16_cache(capi))
+    check_refusals(capi, "ztvm_rope_append", capi.RopeAppendDesc, rope, [(dict(tokens=1 << 24), "tokens")])
+    attention = dict(tokens=(1 << 24) - 1, sequences=1, heads=4, max_query=(1 << 30) - 1, max_kv=(1 << 30) - 1, q_stride=256, out_stride=256, scale=1e30,
+                     q=0x100000, out=1 << 45, query_start=0x4000, kv_length=0x5000, cache=f16_cache(capi))
+    check_refusals(capi, "ztvm_attention", capi.AttentionDesc, attention, [
+        (dict(tokens=1 << 24), "tokens"), (dict(max_query=1 << 30), "max_query"), (dict(max_kv=1 << 30), "max_kv"), (dict(scale=1.1e30), "scale"),
+        (dict(scale=-1.1e30), "scale")])
+    score = dict(rows=(1 << 24) - 1, vocab=100, row_stride=128, inv_temperature=1.0, logits=0x1000)
+    check_refusals(capi, "ztvm_token_logprobs", capi.TokenLogprobsDesc, score, [(dict(rows=1 << 24), "rows")])

@@ -922,9 +922,9 @@ bool mfma_takes(const AttentionArgs& a) {
   const uint64_t at = reinterpret_cast<uint64_t>(c.pages) | c.page_bytes | c.head_bytes | c.side_bytes | c.slot_bytes;
   if (at % 16 || reinterpret_cast<uint64_t>(c.scales) % 4) return false;
   if ((reinterpret_cast<uint64_t>(a.q) | reinterpret_cast<uint64_t>(a.out)) & 15u || a.q_stride % 8 || a.out_stride % 8) return false;
-  // the grid, and key positions a few turns past the last one, stay inside 31 bits
+  // the grid's limits
   const uint64_t rows = (uint64_t)a.max_query * (a.heads / c.kv_heads);
-  return rows <= 64ull * 65535u && a.max_query * (uint64_t)a.heads < (1ull << 31) && a.max_kv < (1u << 30) && (uint64_t)a.sequences * c.kv_heads < (1u << 20);
+  return rows <= 64ull * 65535u && a.max_query * (uint64_t)a.heads < (1ull << 31) && (uint64_t)a.sequences * c.kv_heads < (1u << 20);
 }
 
 struct MfmaPlan {

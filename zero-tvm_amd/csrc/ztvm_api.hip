@@ -836,7 +836,7 @@ int ztvm_rope_append(ztvm_ctx* ctx, const ztvm_rope_append_desc* d) {
   if (!d->qkv || !d->q_out || !d->frequencies || !d->positions || !d->slots) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: null buffer");
   if (((d->qkv | d->q_out) & 1u) || (d->frequencies & 7u) || ((d->positions | d->slots) & 3u))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: misaligned buffer (qkv and q_out 2, frequencies 8, positions and slots 4 bytes)");
-  if (d->tokens >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: too many tokens (%u)", d->tokens);
+  if (d->tokens >= (1u << 24)) return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: too many tokens (%u)", d->tokens);  // a launch holds 2^32 threads
   const bool in_place = d->q_out == d->qkv && d->q_stride == d->qkv_stride;
   if (d->tokens && !in_place && rows_overlap(d->qkv, 2 * width, 2ull * d->qkv_stride, d->q_out, 2 * q_width, 2ull * d->q_stride, d->tokens))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: q_out overlaps qkv (only q_out = qkv with the same stride is allowed)");
@@ -933,7 +933,7 @@ int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
   if (!d->q || !d->out || !d->query_start || !d->kv_length) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: null buffer");
   if (((d->q | d->out) & 1u) || ((d->lse | d->query_start | d->kv_length | d->page_table) & 3u) || (d->tree_mask & 7u))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: misaligned buffer (q and out 2, lse, query_start, kv_length and page_table 4, tree_mask 8 bytes)");
-  if (d->tokens >= (1u << 31) || d->max_query >= (1u << 30) || d->max_kv >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: tokens, max_query or max_kv too large");
+  if (d->tokens >= (1u << 24) || d->max_query >= (1u << 30) || d->max_kv >= (1u << 30)) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: tokens, max_query or max_kv too large");
   if (d->sequences > 65535u) return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: at most 65535 sequences per dispatch (got %u)", d->sequences);
   if (d->page_table) {
     if ((uint64_t)d->page_table_stride * d->cache.page_size < d->max_kv)
@@ -981,7 +981,7 @@ int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* d) {
   if (d->logprob && !d->tokens) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: logprob needs tokens");
   if ((d->logits & (d->logits_f16 ? 1u : 3u)) || ((d->tokens | d->logprob | d->entropy | d->top_ids | d->top_logprobs) & 3u))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: misaligned buffer (logits to their type, the rest 4 bytes)");
-  if (d->rows >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: too many rows (%u)", d->rows);
+  if (d->rows >= (1u << 24)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: too many rows (%u)", d->rows);
   if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
   if (!d->rows) return ZTVM_OK;
   LogprobsArgs a{};
