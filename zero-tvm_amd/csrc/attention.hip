@@ -168,14 +168,14 @@ struct MfmaParams {
   AttentionArgs a;
   float* partial;   // [sequence][head][row of max_query tokens][split][dim], times 2^LIFT
   float2* partial_ml;  // reference value (log2) and sum, times 2^LIFT
-  uint32_t* arrivals;  // of the workgroups that split a row tile, one counter each; zero between launches
+  uint32_t* arrivals;  // of the workgroups that split a row tile, one counter each, zero between launches; null: a launch of its own joins
   uint32_t splits, chunk, group;
   float scale_log2;  // |scale| * log2 e
   uint32_t negate;   // scale < 0: the queries change sign
 };
 
 constexpr float lift_of(bool raw_int8) { return raw_int8 ? 4.f : 9.f; }
-constexpr int MOST_SPLITS = 128;
+constexpr int MOST_SPLITS = 128, FUSED_SPLITS = 16;
 constexpr float NOTHING = -3.0e38f;  // a row's reference value before its first key
 
 __device__ __forceinline__ float across_groups_max(float v) {
@@ -249,7 +249,7 @@ struct MfmaShape {
   static_assert(WIDEN || NS == 1, "only the widened tiles are made of several");
   static_assert(!WIDEN || (RW == 4 && NS == 2), "a wave widens one 16-key block");
   static constexpr int PITCH = DIM + 4;                    // of the joined rows
-  static constexpr int JOIN = KW > 1 ? std::max(KW * ROWS * PITCH * 4 + KW * ROWS * 8, ROWS * MOST_SPLITS * 8) : 0;
+  static constexpr int JOIN = KW > 1 ? std::max(KW * ROWS * PITCH * 4 + KW * ROWS * 8, ROWS * FUSED_SPLITS * 8) : 0;
   static constexpr int LDS = std::max(WIDEN ? 2 * WIDE : STAGES * STAGE, JOIN);
 };
 
@@ -782,6 +782,10 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
       if (parts == 1) {
         finish4(row, d, v, total);
         if (d == 0) finish_row(row, top, total);
+      } else if (!p.arrivals) {  // attention_join_kernel adds the parts
+        const size_t at = partial_at(row) + split;
+        *reinterpret_cast<f4*>(p.partial + at * DIM + d) = v;
+        if (d == 0) p.partial_ml[at] = make_float2(top, total);
       } else {
         const size_t at = partial_at(row) + split;
         put2(p.partial + at * DIM + d, v.x, v.y);
@@ -789,7 +793,7 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
         if (d == 0) put2(reinterpret_cast<float*>(p.partial_ml + at), top, total);
       }
     }
-    if (parts == 1) return;
+    if (parts == 1 || !p.arrivals) return;
     // The workgroup that arrives last adds the parts, in their order. Partial results go past the caches that the XCDs do
     // not share (relaxed device-scope stores and loads), every wave waits for its own stores before the barrier, and one
     // thread counts the arrival; nobody waits for another workgroup.
@@ -839,14 +843,14 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
   }
 }
 
-// Adds the partial results of a row's splits, in their order. One wave per query row and head. BATCH: splits that a lane asks
+// Adds the partial results of a row's splits, in their order. WAVES waves per query row and head. BATCH: splits that a lane asks
 // for at once (few splits: the instructions of an empty batch are what the launch would wait for).
-template <uint32_t BATCH>
+template <uint32_t BATCH, uint32_t WAVES>
 __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t tile_rows, float lift) {
   const AttentionArgs& a = p.a;
   const KvView& c = a.cache;
   const uint32_t lane = threadIdx.x & 63u, b = blockIdx.y;
-  const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 6);  // (row, kv head)
+  const uint32_t wave = threadIdx.x >> 6, unit = WAVES == 4 ? blockIdx.x : blockIdx.x * 4u + wave;  // (row, kv head)
   const uint32_t row = unit / c.kv_heads, h = unit - row * c.kv_heads;
   const int32_t start = a.query_start[b];
   const int64_t n = (int64_t)a.query_start[b + 1] - start;
@@ -863,13 +867,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
   const size_t at = ((size_t)(b * c.kv_heads + h) * a.max_query * p.group + row) * p.splits;
   const float* acc = p.partial + at * c.head_dim;
   const float2* ml = p.partial_ml + at;
-  // a lane takes four dims of every `ways`-th split; the first are asked for before the weights are known
+  // a lane takes four dims of every `steps`-th split; the first are asked for before the weights are known
   const uint32_t quads = c.head_dim / 4, ways = 64u / quads, way = lane / quads, d = (lane - way * quads) * 4;
+  const uint32_t steps = ways * WAVES, first = WAVES == 4 ? wave * ways + way : way;
   f4 x[BATCH];
   auto batch = [&](uint32_t s1) {
 #pragma unroll
     for (uint32_t k = 0; k < BATCH; k++) {
-      const uint32_t s = s1 + k * ways + way;
+      const uint32_t s = s1 + k * steps + first;
       x[k] = s < parts && way < ways ? *reinterpret_cast<const f4*>(acc + (size_t)s * c.head_dim + d) : f4{0.f, 0.f, 0.f, 0.f};
     }
   };
@@ -884,11 +889,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
     const float2 mine = lane < here ? ml[s0 + lane] : make_float2(NOTHING, 0.f);
     const float w = lane < here ? __builtin_amdgcn_exp2f(mine.x - top) : 0.f;
     total += mine.y * w;
-    for (uint32_t s1 = 0; s1 < here; s1 += BATCH * ways) {
+    for (uint32_t s1 = 0; s1 < here; s1 += BATCH * steps) {
       if (s0 + s1) batch(s0 + s1);
 #pragma unroll
       for (uint32_t k = 0; k < BATCH; k++) {
-        const uint32_t s = s1 + k * ways + way;
+        const uint32_t s = s1 + k * steps + first;
         const float ws = __shfl(w, (int)min(s, 63u));
         if (s < 64u) v += x[k] * ws;
       }
@@ -901,6 +906,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
 #pragma unroll
     for (int x = 0; x < 4; x++) other[x] = __shfl(v[x], (int)min(lane + k * quads, 63u));
     sum += other;  // of use in the first way only, where the ways are added in their order
+  }
+  if constexpr (WAVES > 1) {
+    __shared__ f4 of_wave[WAVES][64];
+    of_wave[wave][lane] = sum;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (uint32_t k = 1; k < WAVES; k++) sum += of_wave[k][lane];
   }
   const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
   const uint32_t i = row / p.group, head = h * p.group + (row - i * p.group);
@@ -931,25 +944,37 @@ struct MfmaPlan {
   int qt, rw, kw;
   uint32_t rows, row_tiles, splits, chunk;
   size_t partial_bytes, bytes;
+  bool fused;  // the workgroup that arrives last joins
 };
 MfmaPlan mfma_plan(const AttentionArgs& a) {
   MfmaPlan g{};
   const uint32_t group = a.heads / a.cache.kv_heads;
   const uint64_t rows = (uint64_t)a.max_query * group;
   const bool wide = a.cache.head_dim > 128;
+  // Few rows: the waves of a workgroup split the keys, so that each key is read by one of them (two waves in flight: a batch
+  // of 48 tokens 160 us, four 164). More: four waves share the staged keys and split the rows, two row tiles each where the
+  // registers hold them (int8 trees of up to 64 x 4 rows: one tile a wave 99 us, two 77).
   if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = 2;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
   else g.qt = rows <= 64 || wide ? 1 : 2, g.rw = 4, g.kw = 1;
   g.rows = 16 * g.qt * g.rw;
   g.row_tiles = (uint32_t)((rows + g.rows - 1) / g.rows);
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
-  // enough workgroups for a few rounds of the CUs, none with less than four turns of its waves
+  // Enough workgroups for a few rounds of the CUs. Measured, 512 / 1024 / 2048 of them: a batch of 48 tokens (4000 keys, 32
+  // heads on 8 of 128) - / 164 / 156 us; a tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -; 8 trees over up
+  // to 8200 int8 keys 129 / 81 / 86. None takes fewer keys than two turns of its key waves, or four 64-key turns where the
+  // waves split the rows (one token over 1037 keys, one / two / four / eight turns: 9.9 / 8.9 / 10.0 / 11.5), and a row
+  // has no more than 128 parts: with 256 a step of 8 rows x 8 heads over 64000 keys takes 65.6 instead of 58.3 us, their
+  // join being what grows.
   const uint64_t want = g.rw == 1 ? 2048 : a.sequences == 1 ? 512 : 1024;
   const uint32_t unit = std::max(32u * g.kw, 64u), least = unit * (g.kw > 1 ? 2u : 4u);
   uint64_t splits = (want + groups - 1) / groups;
   splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, (a.max_kv + least - 1) / least, (uint64_t)MOST_SPLITS}));
   g.chunk = (uint32_t)(((a.max_kv + splits - 1) / splits + unit - 1) / unit * unit);
   g.splits = (a.max_kv + g.chunk - 1) / g.chunk;
+  // Few partial rows are joined by the workgroup that arrives last, more by a launch of their own with four waves for each
+  // row: 4 rows x 9 parts 8.9 against 10.7 us, 8 x 8 10.4 and 11.4, but 16 x 32 21.0 and 11.7, 16 x 128 57.8 and 13.7.
+  g.fused = g.kw > 1 && g.splits <= FUSED_SPLITS && rows * g.splits <= 64;
   static_assert(ZTVM_ARRIVALS >= 2048, "a counter for every row tile that is split");
   if (g.splits > 1) {
     const uint64_t n = (uint64_t)a.sequences * a.heads * a.max_query * g.splits;
@@ -967,9 +992,14 @@ hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t
   const dim3 grid(p.a.sequences * p.a.cache.kv_heads * g.splits, g.row_tiles);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * RW * KW), Shape::LDS, s, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || g.splits == 1 || KW > 1) return e;
+  if (e != hipSuccess || g.splits == 1 || p.arrivals) return e;
   const uint32_t units = p.a.max_query * p.a.heads;
-  auto join = g.splits * KD <= 16 ? attention_join_kernel<2> : attention_join_kernel<8>;
+  // many parts: four waves for a row (38 rows x 4 sequences x 128 parts 25.3 -> 23.3 us, 25 x 3 x 128 28.3 -> 22.5)
+  if (g.splits > 16) {
+    hipLaunchKernelGGL((attention_join_kernel<8, 4>), dim3(units, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
+    return hipGetLastError();
+  }
+  auto join = g.splits * KD <= 16 ? attention_join_kernel<2, 1> : attention_join_kernel<8, 1>;
   hipLaunchKernelGGL(join, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
   return hipGetLastError();
 }
@@ -993,6 +1023,7 @@ hipError_t launch_attention(const AttentionArgs& a, void* scratch, uint32_t* arr
     return hipGetLastError();
   }
   const MfmaPlan g = mfma_plan(a);
+  if (!g.fused) arrivals = nullptr;
   MfmaParams p{a, static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + g.partial_bytes), arrivals, g.splits, g.chunk,
                a.heads / a.cache.kv_heads, std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f), a.scale < 0.f};  // never 0: a masked score is -inf times it
   auto by_format = [&](auto kd) {
