@@ -237,7 +237,9 @@ template <int KD, bool INT8, int QT, int RW, int KW, int NS>
 struct MfmaShape {
   static constexpr int DIM = 32 * KD;
   static constexpr int ROWS = 16 * QT * RW;
-  static constexpr int STAGES = RW == 1 ? 2 : 3;
+  // three where four waves meet at a barrier; two for heads of 256, so that two workgroups fit a CU (48 x 2 rows over 9000
+  // keys 44.2 -> 31.8 us)
+  static constexpr int STAGES = RW == 1 || KD > 4 ? 2 : 3;
   static constexpr int KEYS = 32 * NS;
   static constexpr int PART = 32 * DIM * (INT8 ? 2 : 4);  // bytes of 32 keys as they arrive: K then V (int8: rows of K | V)
   static constexpr int SCALES = INT8 ? 256 : 0;
@@ -960,13 +962,16 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   g.rows = 16 * g.qt * g.rw;
   g.row_tiles = (uint32_t)((rows + g.rows - 1) / g.rows);
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
-  // Enough workgroups for a few rounds of the CUs. Measured, 512 / 1024 / 2048 of them: a batch of 48 tokens (4000 keys, 32
-  // heads on 8 of 128) - / 164 / 156 us; a tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -; 8 trees over up
-  // to 8200 int8 keys 129 / 81 / 86. None takes fewer keys than two turns of its key waves, or four 64-key turns where the
-  // waves split the rows (one token over 1037 keys, one / two / four / eight turns: 9.9 / 8.9 / 10.0 / 11.5), and a row
-  // has no more than 128 parts: with 256 a step of 8 rows x 8 heads over 64000 keys takes 65.6 instead of 58.3 us, their
-  // join being what grows.
-  const uint64_t want = g.rw == 1 ? 2048 : a.sequences == 1 ? 512 : 1024;
+  // Workgroups that fill the CUs about once or twice; more cost their beginnings and the join. Measured with 1024 / 1536 /
+  // 2048 where the waves split the keys: 16 sequences x 4000 int8 keys x 8 heads 28.7 / 34.2 / 34.6 us, 4 x 16000 f16
+  // 56.2 / 58.1 / 58.4, and where there are many ragged sequences, whose ends finer parts even out, 48 x up to 4000 162.7 /
+  // 156.4 / 154.8 f16 and 60.6 / 56.3 / 57.7 int8. Heads of 256 leave room for one workgroup a CU: 256 / 512 / 2048 of
+  // them 52.3 / 57.2 / 72.2 us for a token over 27155 keys, 55.7 / 58.8 / 91.5 for 8 x 4000. Waves that split the rows,
+  // 512 / 1024 / 2048: one tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -, 8 ragged int8 trees 126 / 77 / 86.
+  const uint64_t want = wide ? 256 : g.rw == 1 ? (groups > 256 ? 1536 : 1024) : a.sequences == 1 ? 512 : 1024;
+  // A part is two turns of the key waves or more, four 64-key turns where the waves split the rows (one token over 1037
+  // keys, one / two / four / eight turns: 9.9 / 8.9 / 10.0 / 11.5 us), and a row has at most 128: with 256 of them a step
+  // of 8 rows x 8 heads over 64000 keys takes 65.6 instead of 58.3 us, their join being what grows.
   const uint32_t unit = std::max(32u * g.kw, 64u), least = unit * (g.kw > 1 ? 2u : 4u);
   uint64_t splits = (want + groups - 1) / groups;
   splits = std::max<uint64_t>(1, std::min<uint64_t>({splits, (a.max_kv + least - 1) / least, (uint64_t)MOST_SPLITS}));
