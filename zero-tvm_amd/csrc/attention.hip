@@ -142,7 +142,13 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
 //
 // Keys and values travel global -> LDS without passing registers, 32 keys a wave and stage, 16-byte chunks XOR-swizzled
 // so that neither kind of read meets bank conflicts. A page holds a multiple of 16 slots here, so 16 keys always lie in
-// one page and their addresses are one scalar base and a constant per lane.
+// one page and their addresses are one scalar base and a constant per lane. int8 rows that four waves share are fetched
+// into registers instead and widened once for all, 64 keys a turn (transfers and 32 keys: 98 us for the trees below, 77).
+//
+// Measured: 48 tokens of 32 heads over 90 to 8191 f16 keys of 8 x 128, 815 MB: 156 us, 5.2 TB/s, bound by memory, as is a
+// tree of 64 over 65537 keys of 16 x 96 (403 MB, 85 us). 16 trees of 5 to 61 over 200 to 4500 int8 keys of 8 x 128 (87 MB,
+// 21 GFLOP): 77 us, bound by the issue of vector instructions: 480 a wave and turn beside 64 matrix instructions. A token
+// over 1037 keys: 8.9 us, a chain of dependent steps.
 
 // chunk swizzles. A row of `KD` 64-byte units starts at bank slot 4*KD*row mod 16 (16 slots of 16 bytes): the XOR supplies
 // the row bits that the pitch does not.
@@ -955,7 +961,8 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   const bool wide = a.cache.head_dim > 128;
   // Few rows: the waves of a workgroup split the keys, so that each key is read by one of them (two waves in flight: a batch
   // of 48 tokens 160 us, four 164). More: four waves share the staged keys and split the rows, two row tiles each where the
-  // registers hold them (int8 trees of up to 64 x 4 rows: one tile a wave 99 us, two 77).
+  // registers hold them (int8 trees of up to 61 x 4 rows: one tile a wave 99 us, two 77; heads of
+  // 256 spill with two: 15 trees of 74 rows over 1846 int8 keys 108 us, with two 158).
   if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = 2;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
   else g.qt = rows <= 64 || wide ? 1 : 2, g.rw = 4, g.kw = 1;
@@ -964,10 +971,10 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   const uint64_t groups = (uint64_t)a.sequences * a.cache.kv_heads * g.row_tiles;
   // Workgroups that fill the CUs about once or twice; more cost their beginnings and the join. Measured with 1024 / 1536 /
   // 2048 where the waves split the keys: 16 sequences x 4000 int8 keys x 8 heads 28.7 / 34.2 / 34.6 us, 4 x 16000 f16
-  // 56.2 / 58.1 / 58.4, and where there are many ragged sequences, whose ends finer parts even out, 48 x up to 4000 162.7 /
-  // 156.4 / 154.8 f16 and 60.6 / 56.3 / 57.7 int8. Heads of 256 leave room for one workgroup a CU: 256 / 512 / 2048 of
+  // 56.2 / 58.1 / 58.4, and where there are many ragged sequences, whose ends finer parts even out, 48 x up to 8191 f16
+  // 162.7 / 156.4 / 154.8, x up to 4000 int8 60.6 / 56.3 / 57.7. Heads of 256 leave room for one workgroup a CU: 256 / 512 / 2048 of
   // them 52.3 / 57.2 / 72.2 us for a token over 27155 keys, 55.7 / 58.8 / 91.5 for 8 x 4000. Waves that split the rows,
-  // 512 / 1024 / 2048: one tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -, 8 ragged int8 trees 126 / 77 / 86.
+  // 512 / 1024 / 2048: one tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -, 16 ragged int8 trees 126 / 77 / 86.
   const uint64_t want = wide ? 256 : g.rw == 1 ? (groups > 256 ? 1536 : 1024) : a.sequences == 1 ? 512 : 1024;
   // A part is two turns of the key waves or more, four 64-key turns where the waves split the rows (one token over 1037
   // keys, one / two / four / eight turns: 9.9 / 8.9 / 10.0 / 11.5 us), and a row has at most 128: with 256 of them a step

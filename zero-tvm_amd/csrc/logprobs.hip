@@ -94,7 +94,9 @@ __global__ __launch_bounds__(256) void logprobs_any_kernel(const LogprobsArgs p)
 // maximum, sum and weighted sum, and the maximum of each neighbourhood (two loads of the wave: 512 f32 or 1024 f16
 // logits that lie side by side). The best top_k logits lie in the top_k neighbourhoods with the largest maxima (ties:
 // the lower one), so the joining workgroup looks at those again and at nothing else. Bound by the one read of the logits
-// where there are many rows, by the chain of dependent steps behind it where there are few.
+// where there are many rows (384 rows of 248320 f32, 381 MB: 65 us for the read, 5.8 TB/s, and 10 for the join), by the
+// chain of dependent steps behind it where there are few (one row of 128000 f32: 3.6 us and 7.8). Both in one launch, a
+// workgroup of 1024 threads a row, took 151 us for the 384 rows and is not faster for one.
 constexpr int GROUPS = 8;
 constexpr int HOODS = GROUPS / 2;          // neighbourhoods of a segment
 constexpr uint32_t MAX_HOODS = 4096;       // of a row
@@ -451,7 +453,8 @@ hipError_t launch_typed(const LogprobsArgs& a, void* scratch, hipStream_t s) {
   SegmentStats* stats = static_cast<SegmentStats*>(scratch);
   const uint64_t waves = (uint64_t)a.rows * segments;
   hipLaunchKernelGGL(logits_segments_kernel<T>, dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, s, a, stats, segments, c);
-  // few rows: as many waves as a row can use; many: as many rows as fit
+  // few rows: as many waves as a row can use; many: as many rows as fit (1024 / 256 threads: a row of
+  // 128000 logits 11.0 / 12.4 us; of 32000, 256 rows 15.6 / 17.3, 512 21.9 / 22.5, 700 30.2 / 27.0, 2048 75.9 / 63.8)
   if (a.rows <= 512) hipLaunchKernelGGL((logits_answer_kernel<T, 1024>), dim3(a.rows), dim3(1024), 0, s, a, stats, segments, c);
   else hipLaunchKernelGGL((logits_answer_kernel<T, 256>), dim3(a.rows), dim3(256), 0, s, a, stats, segments, c);
   return hipGetLastError();
