@@ -328,7 +328,8 @@ ZTVM_API int ztvm_moe_slot_translate(ztvm_ctx* ctx, uint64_t ids_out, uint64_t i
 /* A paged cache as ztvm_qkv_fused (F16) or ztvm_kv_quantize_int8 (INT8) writes it. */
 enum {
   ZTVM_KV_F16 = 0, /* element page*kv_page_stride + head*head_page_stride + slot*head_dim + dim (+ v_page_offset for V) */
-  ZTVM_KV_INT8 = 1 /* word page . head . slot . side(K, V) . dim/4, and one f16 scale page . head . slot . side */
+  ZTVM_KV_INT8 = 1 /* word page . head . slot . side(K, V) . dim/4, and one f16 scale page . head . slot . side (of f16
+                    * rows: at most 516) */
 };
 typedef struct ztvm_kv_cache {
   uint32_t format; /* ZTVM_KV_* */
@@ -408,7 +409,7 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen. The work is
  * split over workgroups by these bounds, so bounds near the lengths are the fast ones. Scratch for the joined partial
  * results comes from the context and depends on the descriptor only.
- * Head sizes of 64, 96, 128 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
+ * Head sizes of 32, 64, 96, 128, 160, 192 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
  * cores; everything else is right as well, by a plain kernel. */
 typedef struct ztvm_attention_desc {
   uint32_t tokens;    /* rows of q, out, lse and tree_mask; below 2^24 */

@@ -427,6 +427,24 @@ def test_recordings_that_share_the_scratch(ctx, capi):
             ctx.cmdbuf_destroy(r)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dim", [32, 160, 192, 224])
+@pytest.mark.parametrize("queries", [1, 6, 40])
+def test_other_head_sizes(ctx, capi, dim, queries, int8):
+    """Heads of a multiple of 32, in every shape of workgroup, over one part of the keys and many."""
+    Step(dim + queries, 8, 2, dim, 16, [(queries, 2100), (queries, 300), (queries, 47)], int8, tree="tree").check(ctx, capi)
+
+
+@pytest.mark.parametrize("dim,queries", [(32, 5), (160, 5), (192, 5), (160, 40)])
+def test_infinities_in_masked_places_of_other_head_sizes(ctx, capi, dim, queries):
+    s = Step(dim, 4, 2, dim, 16, [(queries, 100)])
+    for page in range(s.cache.shape[0]):
+        if page not in s.table[0, :7]:
+            s.cache[page] = np.inf
+    s.cache[s.table[0, 6], :, :, 4:] = np.nan           # behind the last position
+    s.check(ctx, capi)
+
+
 def test_two_contexts_at_once(ctx, capi):
     """Two contexts on one GPU, their dispatches in flight together: scratch and counters are each one's own."""
     a, b = Step(27, 8, 2, 128, 16, [(1, 4000), (1, 3000)]), Step(28, 8, 2, 128, 16, [(1, 2500), (1, 3999)])
