@@ -243,7 +243,7 @@ template <int KD, bool INT8, int QT, int RW, int KW, int NS>
 struct MfmaShape {
   static constexpr int DIM = 32 * KD;
   static constexpr int ROWS = 16 * QT * RW;
-  // three where four waves meet at a barrier; two for heads of 256, so that two workgroups fit a CU (48 x 2 rows over 9000
+  // three where four waves meet at a barrier; two for heads past 128, so that two workgroups fit a CU (48 x 2 rows over 9000
   // keys 44.2 -> 31.8 us)
   static constexpr int STAGES = RW == 1 || KD > 4 ? 2 : 3;
   static constexpr int KEYS = 32 * NS;
@@ -973,7 +973,7 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   // Workgroups that fill the CUs about once or twice; more cost their beginnings and the join. Measured with 1024 / 1536 /
   // 2048 where the waves split the keys: 16 sequences x 4000 int8 keys x 8 heads 28.7 / 34.2 / 34.6 us, 4 x 16000 f16
   // 56.2 / 58.1 / 58.4, and where there are many ragged sequences, whose ends finer parts even out, 48 x up to 8191 f16
-  // 162.7 / 156.4 / 154.8, x up to 4000 int8 60.6 / 56.3 / 57.7. Heads of 256 leave room for one workgroup a CU: 256 / 512 / 2048 of
+  // 162.7 / 156.4 / 154.8, x up to 4000 int8 60.6 / 56.3 / 57.7. Heads past 128 leave room for one workgroup a CU; of 256: 256 / 512 / 2048 of
   // them 52.3 / 57.2 / 72.2 us for a token over 27155 keys, 55.7 / 58.8 / 91.5 for 8 x 4000. Waves that split the rows,
   // 512 / 1024 / 2048: one tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -, 16 ragged int8 trees 126 / 77 / 86.
   const uint64_t want = wide ? 256 : g.rw == 1 ? (groups > 256 ? 1536 : 1024) : a.sequences == 1 ? 512 : 1024;
