@@ -406,8 +406,8 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  * sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
  * matter. Rows outside every sequence are left as they were.
  * max_query and max_kv bound n_b and kv_length[b] (the lengths are read on the device, so a recorded step can be
- * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen. The work is
- * split over workgroups by these bounds, so bounds near the lengths are the fast ones. Scratch for the joined partial
+ * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen (context still
+ * goes by kv_length[b]). The work is split over workgroups by these bounds, so bounds near the lengths are the fast ones. Scratch for the joined partial
  * results comes from the context and depends on the descriptor only.
  * Head sizes of 32, 64, 96, 128, 160, 192 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
  * cores; everything else is right as well, by a plain kernel. */

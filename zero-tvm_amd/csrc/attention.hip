@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
   if (!find_sequence(p, (int32_t)t, b, i, n)) return;
   const KvView& c = p.cache;
   const uint32_t dim = c.head_dim, kvh = h / (p.heads / c.kv_heads);
-  const int32_t length = min(max(p.kv_length[b], 0), (int32_t)p.max_kv);
-  const int64_t context = (int64_t)length - n;
+  const int32_t cached = max(p.kv_length[b], 0), length = min(cached, (int32_t)p.max_kv);
+  const int64_t context = (int64_t)cached - n;  // by all that is cached: the bound hides positions and moves none
   for (uint32_t d = tid; d < dim; d += 256u) q[d] = (float)p.q[(size_t)t * p.q_stride + (size_t)h * dim + d];
   // the product: `groups` groups of threads share the keys of a tile, a thread takes dims d0, d0 + 256
   uint32_t width = 1;
@@ -298,8 +298,8 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
   const uint32_t row0 = blockIdx.y * ROWS;
   if (start < 0 || tokens <= 0 || row0 >= tokens * p.group) return;
   const uint32_t rows = (uint32_t)tokens * p.group;
-  const int32_t length = min(max(a.kv_length[b], 0), (int32_t)a.max_kv);
-  const int64_t context = length - n;
+  const int32_t cached = max(a.kv_length[b], 0), length = min(cached, (int32_t)a.max_kv);
+  const int64_t context = cached - n;  // by all that is cached: the bound hides positions and moves none
   const bool tree = a.tree_mask != nullptr;
   const uint32_t last_row = min(row0 + ROWS, rows) - 1;
   const int64_t seen_by_all = tree ? context : context + row0 / p.group + 1;
@@ -864,8 +864,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
   const int64_t n = (int64_t)a.query_start[b + 1] - start;
   const int64_t tokens = min(min(n, (int64_t)a.max_query), (int64_t)a.tokens - start);
   if (start < 0 || tokens <= 0 || row >= tokens * p.group) return;
-  const int32_t length = min(max(a.kv_length[b], 0), (int32_t)a.max_kv);
-  const int64_t context = length - n;
+  const int32_t cached = max(a.kv_length[b], 0), length = min(cached, (int32_t)a.max_kv);
+  const int64_t context = cached - n;
   // how many splits the row's workgroup had, as it worked it out
   const uint32_t last_row = min(row / tile_rows * tile_rows + tile_rows, (uint32_t)tokens * p.group) - 1;
   const int64_t seen_by_any = a.tree_mask ? length : context + last_row / p.group + 1;
