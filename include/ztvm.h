@@ -402,8 +402,10 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  *   tree_mask:       p < context, or bit (p - context) of its mask_words 64-bit words is set        (a tree)
  * and p's page is inside the cache. Query head h reads kv head h / (heads/kv_heads).
  *   out[t,h] = sum_p softmax_p(scale * q[t,h].k[p]) * v[p],   lse[t,h] = ln sum_p exp(scale * q[t,h].k[p])
- * Sums are f32, the probabilities enter the product as f16 (relative 2^-11 each), out rounds once to f16. A token that
- * sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
+ * Sums are f32, out rounds once to f16. What multiplies the cached values enters that product as f16: the probability, or
+ * for INT8 the probability times the value's scale. Each is off by 2^-11 of itself or by 2^-34 of the row's largest,
+ * whichever is more (INT8 where more than 32 rows share a kv head: of the largest probability times the scale at hand, which
+ * counts as 2^-13 at least). A token that sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
  * matter. Rows outside every sequence are left as they were.
  * max_query and max_kv bound n_b and kv_length[b] (the lengths are read on the device, so a recorded step can be
  * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen (context still

@@ -134,11 +134,14 @@ __global__ __launch_bounds__(256) void attention_any_kernel(const AttentionArgs 
 //                 reads deliver from rows of V as they lie in the cache (ds_read_b64_tr_b16 takes 4 keys x 16 dims a
 //                 group of 16 lanes, ds_read_b64_tr_b8 8 keys x 16 dims), so nothing is shuffled between the products.
 //
-// The running maximum is lazy: a row's reference value moves only when a score exceeds it by 2^THR, so most tiles need no
-// exchange between lanes and no rescaling. Probabilities are lifted by 2^LIFT before they round to f16, which keeps
-// small ones out of its subnormal range; int8 keys' scales multiply the scores, int8 values' scales the probabilities
-// (their power of two goes into the widened values where those are made once for several waves: exact, and the
-// probabilities keep their range).
+// The running maximum is lazy: a row's reference value moves only when what enters the second product passes CAP, so most
+// tiles need no exchange between lanes and no rescaling. Probabilities are lifted by 2^LIFT before they round to f16, which
+// keeps those within 2^-23 of the largest out of its subnormal range. int8 keys' scales multiply the scores, int8 values'
+// scales the probabilities. Where the values are widened once for several waves, the scale's power of two goes into them
+// (exact) and the rest, 1 to 2, into the probabilities. Where a wave widens its own, the whole scale goes into the
+// probabilities and the reference follows their products: it is the largest score plus log2 of its key's scale, so that the
+// products use f16's range however small the values are. The f32 sum of the probabilities has range for that: they are at
+// most 2^24 times CAP.
 //
 // Keys and values travel global -> LDS without passing registers, 32 keys a wave and stage, 16-byte chunks XOR-swizzled
 // so that neither kind of read meets bank conflicts. A page holds a multiple of 16 slots here, so 16 keys always lie in
@@ -180,7 +183,8 @@ struct MfmaParams {
   uint32_t negate;   // scale < 0: the queries change sign
 };
 
-constexpr float lift_of(bool raw_int8) { return raw_int8 ? 4.f : 9.f; }
+constexpr float LIFT = 9.f, CAP = 32768.f;  // log2; what enters the second product is LIFT above the reference and at most CAP
+constexpr float LEAST_SCALE = 0x1p-24f;     // of f16: what a value scale of zero counts as where the reference is found
 constexpr int MOST_SPLITS = 128, FUSED_SPLITS = 16;
 constexpr float NOTHING = -3.0e38f;  // a row's reference value before its first key
 
@@ -273,10 +277,7 @@ template <int KD, bool INT8, int QT, int RW, int KW, int NS>
 __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS == 1 ? 4 : 2) void attention_mfma_kernel(const MfmaParams p) {
   using Shape = MfmaShape<KD, INT8, QT, RW, KW, NS>;
   constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, ST = Shape::STAGES, KEYS = Shape::KEYS;
-  // probabilities enter f16 times 2^LIFT and stay below 2^(THR + LIFT): inside f16's range. Where int8 scales multiply them
-  // as they are, times 515 more (the largest scale whose 127 counts f16 can hold).
   constexpr bool RAW8 = INT8 && !Shape::WIDEN;
-  constexpr float LIFT = lift_of(RAW8), CAP = RAW8 ? 64.f : 32768.f;  // CAP = 2^(THR + LIFT)
   constexpr int MOVES = INT8 ? KD * 2 : KD * 4;     // transfers of 1 KiB that bring 32 keys
   constexpr int MOVES_EACH = (MOVES + RW - 1) / RW;  // of which a wave makes so many (the last one twice where they do not share evenly)
   constexpr int DMA = MOVES_EACH + (INT8 ? 1 : 0);   // and the scales
@@ -495,6 +496,15 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
       odd = __builtin_amdgcn_readfirstlane(odd);
       asm volatile("" : "+s"(odd));  // a condition of its own: tied to `edge` the compiler doubles the code behind it
     }
+    float raw[RAW8 ? H : 1][4], size[RAW8 ? H : 1][4];  // the value scales and their magnitudes within f16's numbers but zero
+    if constexpr (RAW8) {
+#pragma unroll
+      for (int half = 0; half < H; half++) {
+        scale_of(half, true, raw[half]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) size[half][i] = fminf(fmaxf(fabsf(raw[half][i]), LEAST_SCALE), 65504.f);
+      }
+    }
     h8 pf[QT][NS];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -527,14 +537,18 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
 #pragma unroll
       for (int half = 0; half < H; half++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) most = fmaxf(most, e[half][i]);
+        for (int i = 0; i < 4; i++) {
+          if constexpr (RAW8) most = fmaxf(most, e[half][i] * size[half][i]);
+          else most = fmaxf(most, e[half][i]);
+        }
       if (__any(most > CAP)) {
         float top = -INFINITY;
 #pragma unroll
         for (int half = 0; half < H; half++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const float x = s[t][half][i] * units;
+            float x = s[t][half][i] * units;
+            if constexpr (RAW8) x += __builtin_amdgcn_logf(size[half][i]);
             top = fmaxf(top, !edge || sees(half, i) ? x : -INFINITY);
           }
         const float next = fmaxf(m[t], across_groups_max(top));
@@ -548,9 +562,10 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
 #pragma unroll
       for (int half = 0; half < H; half++) {
         float vs[4] = {1.f, 1.f, 1.f, 1.f};
-        if constexpr (INT8) scale_of(half, true, vs);
+        if constexpr (Shape::WIDEN) scale_of(half, true, vs);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
+          if constexpr (RAW8) vs[i] = raw[half][i];
           l[t] += e[half][i];
           pf[t][half / 2][4 * (half & 1) + i] = (_Float16)(INT8 ? e[half][i] * vs[i] : e[half][i]);
         }
@@ -854,7 +869,7 @@ __global__ __launch_bounds__(64 * RW * KW, KD > 4 ? 1 : RW > 1 && QT == 1 && NS 
 // Adds the partial results of a row's splits, in their order. WAVES waves per query row and head. BATCH: splits that a lane asks
 // for at once (few splits: the instructions of an empty batch are what the launch would wait for).
 template <uint32_t BATCH, uint32_t WAVES>
-__global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t tile_rows, float lift) {
+__global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p, uint32_t tile_rows) {
   const AttentionArgs& a = p.a;
   const KvView& c = a.cache;
   const uint32_t lane = threadIdx.x & 63u, b = blockIdx.y;
@@ -931,7 +946,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const MfmaParams p,
     for (int x = 0; x < 4; x++) o[x] = narrow_f32(sum[x] * inv);
     *reinterpret_cast<h4*>(a.out + (size_t)(start + i) * a.out_stride + (size_t)head * c.head_dim + d) = o;
   }
-  if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top - lift + __log2f(total)) * 0.69314718055994531f : -INFINITY;
+  if (a.lse && lane == 0) a.lse[(size_t)(start + i) * a.heads + head] = total > 0.f || total != total ? (top - LIFT + __log2f(total)) * 0.69314718055994531f : -INFINITY;
 }
 
 // What the matrix-core kernel takes: whole 64-byte units of a head, pages of whole 16-key blocks, 16-byte rows. (A token over
@@ -1009,11 +1024,11 @@ hipError_t launch_mfma_shape(const MfmaParams& p, const MfmaPlan& g, hipStream_t
   const uint32_t units = p.a.max_query * p.a.heads;
   // many parts: four waves for a row (38 rows x 4 sequences x 128 parts 25.3 -> 23.3 us, 25 x 3 x 128 28.3 -> 22.5)
   if (g.splits > 16) {
-    hipLaunchKernelGGL((attention_join_kernel<8, 4>), dim3(units, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
+    hipLaunchKernelGGL((attention_join_kernel<8, 4>), dim3(units, p.a.sequences), dim3(256), 0, s, p, g.rows);
     return hipGetLastError();
   }
   auto join = g.splits * KD <= 16 ? attention_join_kernel<2, 1> : attention_join_kernel<8, 1>;
-  hipLaunchKernelGGL(join, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows, lift_of(INT8 && !Shape::WIDEN));
+  hipLaunchKernelGGL(join, dim3((units + 3) / 4, p.a.sequences), dim3(256), 0, s, p, g.rows);
   return hipGetLastError();
 }
 template <int KD, bool INT8>
