@@ -73,7 +73,7 @@ __device__ __forceinline__ void wait_vm() {
 }
 template <int N>
 __device__ __forceinline__ void wait_lgkm() {
-  asm volatile("s_waitcnt lgkmcnt(%0)" : : "n"(N));
+  asm volatile("s_waitcnt lgkmcnt(%0)" : : "n"(N) : "memory");
 }
 // wait until at most N younger fetches are in flight, then release v
 template <int N, class T>
