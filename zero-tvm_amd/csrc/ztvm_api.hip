@@ -359,7 +359,8 @@ int cache_view(const ztvm_kv_cache* c, KvView* v, char* why, size_t n) {
 // Whether [a, a + rows of a_width every a_stride] and the like at b share a byte other than by being the same array:
 // two column windows of one wider array (equal strides, columns apart) do not.
 bool rows_overlap(uint64_t a, uint64_t a_width, uint64_t a_stride, uint64_t b, uint64_t b_width, uint64_t b_stride, uint64_t rows) {
-  const uint64_t a_end = a + (rows - 1) * a_stride + a_width, b_end = b + (rows - 1) * b_stride + b_width;
+  typedef unsigned __int128 wide;  // 2^31 rows of the largest stride end past 64 bits
+  const wide a_end = (wide)a + (wide)(rows - 1) * a_stride + a_width, b_end = (wide)b + (wide)(rows - 1) * b_stride + b_width;
   if (a_end <= b || b_end <= a) return false;
   if (a_stride != b_stride) return true;
   const uint64_t lo = a < b ? a : b, hi = a < b ? b : a, lo_width = a < b ? a_width : b_width, hi_width = a < b ? b_width : a_width;
