@@ -323,7 +323,9 @@ ZTVM_API int ztvm_moe_slot_translate(ztvm_ctx* ctx, uint64_t ids_out, uint64_t i
  * device memory (positions, slots, page numbers, lengths) is checked in the kernel, so a bad one cannot fault the
  * GPU; the descriptors are checked before anything is enqueued, and before the context is looked at, so that a
  * descriptor can be tried with a null context on a machine without a GPU ("null context" is then the only
- * complaint left). All may be recorded. */
+ * complaint left). An output that overlaps another array of the call, the cache that it reads or writes among them, is
+ * refused unless it says otherwise below (arrays that lie between the rows of another are apart); the cache that
+ * ztvm_rope_append writes and its frequencies, positions and slots are the caller's to keep apart. All may be recorded. */
 
 /* A paged cache as ztvm_qkv_fused (F16) or ztvm_kv_quantize_int8 (INT8) writes it. */
 enum {

@@ -368,6 +368,55 @@ bool rows_overlap(uint64_t a, uint64_t a_width, uint64_t a_stride, uint64_t b, u
   return !(col >= lo_width && col + hi_width <= a_stride);
 }
 
+// An array of a dispatch: `count` rows of `width` bytes, `stride` apart, from `at` to `end` (where 64 bits end at the latest).
+// A null or empty one is from 0 to 0 and overlaps nothing.
+struct Region {
+  const char* name;
+  uint64_t at, end, width, stride, count;
+};
+Region rows_of(const char* name, uint64_t at, uint64_t width, uint64_t stride, uint64_t count) {
+  if (!at || !width || !count) return Region{name, 0, 0, 1, 1, 0};
+  uint64_t span, end;
+  if (__builtin_mul_overflow(count - 1, stride, &span) || __builtin_add_overflow(span, width, &span) || __builtin_add_overflow(at, span, &end)) end = ~0ull;
+  return Region{name, at, end, width, stride, count};
+}
+Region flat(const char* name, uint64_t at, uint64_t bytes) { return rows_of(name, at, bytes, bytes, 1); }
+
+// Whether a row of `a` shares a byte with [b, b_end): the first row that ends past b is the one to look at.
+bool touches(const Region& a, uint64_t b, uint64_t b_end) {
+  const uint64_t i = a.at + a.width > b ? 0 : (b - a.at - a.width) / a.stride + 1;
+  return i < a.count && (unsigned __int128)i * a.stride + a.at < b_end;
+}
+bool regions_overlap(const Region& a, const Region& b) {
+  if (a.end <= b.at || b.end <= a.at) return false;  // the rule: what follows is for an array between the rows of another, or a mistake
+  if (b.count == 1) return touches(a, b.at, b.end);
+  if (a.count == 1) return touches(b, a.at, a.end);
+  const Region &few = a.count < b.count ? a : b, &many = a.count < b.count ? b : a;
+  for (uint64_t i = 0; i < few.count; i++)
+    if (touches(many, few.at + i * few.stride, few.at + i * few.stride + few.width)) return true;
+  return false;
+}
+// The first of the outputs that overlaps one of the inputs or a later output, and what it overlaps.
+bool find_overlap(const Region* out, size_t outs, const Region* in, size_t ins, const char** which, const char** with) {
+  for (size_t i = 0; i < outs; i++)
+    for (size_t k = 0; k < outs - i - 1 + ins; k++) {
+      const Region& other = k < outs - i - 1 ? out[i + 1 + k] : in[k - (outs - i - 1)];
+      if (!regions_overlap(out[i], other)) continue;
+      *which = out[i].name;
+      *with = other.name;
+      return true;
+    }
+  return false;
+}
+// What a dispatch touches of a cache: its whole pages and their scales.
+Region pages_of(const KvView& c) {
+  const uint64_t used = c.int8 ? c.page_bytes : c.side_bytes + c.kv_heads * c.head_bytes;
+  return rows_of("the cache's pages", reinterpret_cast<uint64_t>(c.pages), used, c.page_bytes, c.num_pages);
+}
+Region scales_of(const KvView& c) {
+  return c.int8 ? flat("the cache's scales", reinterpret_cast<uint64_t>(c.scales), 4ull * c.kv_heads * c.page_size * c.num_pages) : rows_of("", 0, 0, 0, 0);
+}
+
 struct Option {
   const char* name;
   int Tune::*field;
@@ -841,6 +890,13 @@ int ztvm_rope_append(ztvm_ctx* ctx, const ztvm_rope_append_desc* d) {
   const bool in_place = d->q_out == d->qkv && d->q_stride == d->qkv_stride;
   if (d->tokens && !in_place && rows_overlap(d->qkv, 2 * width, 2ull * d->qkv_stride, d->q_out, 2 * q_width, 2ull * d->q_stride, d->tokens))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: q_out overlaps qkv (only q_out = qkv with the same stride is allowed)");
+  const Region q_rows = rows_of("q_out", d->q_out, 2 * q_width, 2ull * d->q_stride, d->tokens), qkv_rows = rows_of("qkv", d->qkv, 2 * width, 2ull * d->qkv_stride, d->tokens);
+  const Region stored[] = {pages_of(a.cache), scales_of(a.cache)};
+  const Region read[] = {stored[0], stored[1], flat("frequencies", d->frequencies, 4ull * d->rotary_dim), flat("positions", d->positions, 4ull * d->tokens),
+                         flat("slots", d->slots, 4ull * d->tokens)};
+  const char *which, *with;
+  if (find_overlap(&q_rows, 1, read, 5, &which, &with) || find_overlap(&qkv_rows, 1, stored, 2, &which, &with))
+    return fail(ctx, ZTVM_E_INVALID, "ztvm_rope_append: %s overlaps %s", which, with);
   if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
   if (!d->tokens) return ZTVM_OK;
   a.qkv = reinterpret_cast<const _Float16*>(d->qkv);
@@ -907,6 +963,10 @@ int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* d) {
   if (d->tokens >= (1u << 31)) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: too many tokens (%u)", d->tokens);
   if (d->tokens && d->k_out && d->v_out && rows_overlap(d->k_out, 2 * width, 2ull * d->out_stride, d->v_out, 2 * width, 2ull * d->out_stride, d->tokens))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: k_out and v_out overlap");
+  const Region read[] = {pages_of(a.cache), scales_of(a.cache), flat("slots", d->slots, 4ull * d->tokens)};
+  const char *which, *with;
+  for (const Region& rows : {rows_of("k_out", d->k_out, 2 * width, 2ull * d->out_stride, d->tokens), rows_of("v_out", d->v_out, 2 * width, 2ull * d->out_stride, d->tokens)})
+    if (find_overlap(&rows, 1, read, 3, &which, &with)) return fail(ctx, ZTVM_E_INVALID, "ztvm_kv_read: %s overlaps %s", which, with);
   if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
   if (!d->tokens) return ZTVM_OK;
   a.k_out = reinterpret_cast<_Float16*>(d->k_out);
@@ -946,6 +1006,17 @@ int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* d) {
     return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: mask_words=%u hold less than max_query=%u bits", d->mask_words, d->max_query);
   if (d->tokens && d->sequences && rows_overlap(d->q, 2 * width, 2ull * d->q_stride, d->out, 2 * width, 2ull * d->out_stride, d->tokens))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: out overlaps q");
+  if (d->tokens && d->sequences && d->max_query) {
+    const uint64_t pages = ((uint64_t)d->max_kv + d->cache.page_size - 1) / d->cache.page_size;  // of a sequence's row in the table
+    const Region written[] = {flat("lse", d->lse, 4ull * d->tokens * d->heads), rows_of("out", d->out, 2 * width, 2ull * d->out_stride, d->tokens)};
+    const Region read[] = {flat("query_start", d->query_start, 4ull * d->sequences + 4), flat("kv_length", d->kv_length, 4ull * d->sequences),
+                           rows_of("page_table", d->page_table, 4 * pages, 4ull * d->page_table_stride, d->sequences),
+                           flat("tree_mask", d->tree_mask, 8ull * d->tokens * d->mask_words), pages_of(a.cache), scales_of(a.cache)};
+    const Region q_rows = rows_of("q", d->q, 2 * width, 2ull * d->q_stride, d->tokens);
+    const char *which, *with;
+    if (find_overlap(written, 2, read, 6, &which, &with) || find_overlap(written, 1, &q_rows, 1, &which, &with))
+      return fail(ctx, ZTVM_E_INVALID, "ztvm_attention: %s overlaps %s", which, with);
+  }
   if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
   if (!d->tokens || !d->sequences || !d->max_query) return ZTVM_OK;
   a.q = reinterpret_cast<const _Float16*>(d->q);
@@ -983,6 +1054,12 @@ int ztvm_token_logprobs(ztvm_ctx* ctx, const ztvm_token_logprobs_desc* d) {
   if ((d->logits & (d->logits_f16 ? 1u : 3u)) || ((d->tokens | d->logprob | d->entropy | d->top_ids | d->top_logprobs) & 3u))
     return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: misaligned buffer (logits to their type, the rest 4 bytes)");
   if (d->rows >= (1u << 24)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: too many rows (%u)", d->rows);
+  const uint64_t element = d->logits_f16 ? 2 : 4, best = 4ull * d->rows * d->top_k;
+  const Region written[] = {flat("logprob", d->logprob, 4ull * d->rows), flat("entropy", d->entropy, 4ull * d->rows), flat("top_ids", d->top_ids, best),
+                            flat("top_logprobs", d->top_logprobs, best)};
+  const Region read[] = {rows_of("logits", d->logits, element * d->vocab, element * d->row_stride, d->rows), flat("tokens", d->logprob ? d->tokens : 0, 4ull * d->rows)};
+  const char *which, *with;
+  if (find_overlap(written, 4, read, 2, &which, &with)) return fail(ctx, ZTVM_E_INVALID, "ztvm_token_logprobs: %s overlaps %s", which, with);
   if (!ctx) return fail(nullptr, ZTVM_E_INVALID, "null context");
   if (!d->rows) return ZTVM_OK;
   LogprobsArgs a{};
