@@ -4,6 +4,7 @@
 // Every failure becomes a JS exception carrying ztvm_last_error().
 #include <node_api.h>
 
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
@@ -609,15 +610,24 @@ bool read_fields(napi_env env, napi_value obj, const Field* fields, size_t n, vo
     if (!has) continue;
     napi_get_named_property(env, obj, f.name, &v);
     double number = 0;
-    bool ok = true;
-    if (f.kind == 'u') ok = napi_get_value_uint32(env, v, reinterpret_cast<uint32_t*>(at)) == napi_ok;
-    else if (f.kind == 'f') ok = napi_get_value_double(env, v, &number) == napi_ok;
-    else if (!get_u64(env, v, reinterpret_cast<uint64_t*>(at))) return false;
-    if (!ok) {
+    if (f.kind == 'a') {
+      if (!get_u64(env, v, reinterpret_cast<uint64_t*>(at))) return false;
+      continue;
+    }
+    if (napi_get_value_double(env, v, &number) != napi_ok) {
       napi_throw_type_error(env, nullptr, (std::string("ztvm addon: descriptor field '") + f.name + "' must be a number").c_str());
       return false;
     }
-    if (f.kind == 'f') *reinterpret_cast<float*>(at) = static_cast<float>(number);
+    if (f.kind == 'f') {
+      *reinterpret_cast<float*>(at) = static_cast<float>(number);
+      continue;
+    }
+    // a count that is no whole number of 32 bits would be taken modulo 2^32, NaN as 0
+    if (!(number >= 0 && number <= 4294967295.0 && number == std::floor(number))) {
+      napi_throw_range_error(env, nullptr, (std::string("ztvm addon: descriptor field '") + f.name + "' must be a whole number below 2^32").c_str());
+      return false;
+    }
+    *reinterpret_cast<uint32_t*>(at) = static_cast<uint32_t>(number);
   }
   return true;
 }
