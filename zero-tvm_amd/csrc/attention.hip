@@ -989,9 +989,16 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   // 2048 where the waves split the keys: 16 sequences x 4000 int8 keys x 8 heads 28.7 / 34.2 / 34.6 us, 4 x 16000 f16
   // 56.2 / 58.1 / 58.4, and where there are many ragged sequences, whose ends finer parts even out, 48 x up to 8191 f16
   // 162.7 / 156.4 / 154.8, x up to 4000 int8 60.6 / 56.3 / 57.7. Heads past 128 leave room for one workgroup a CU; of 256: 256 / 512 / 2048 of
-  // them 52.3 / 57.2 / 72.2 us for a token over 27155 keys, 55.7 / 58.8 / 91.5 for 8 x 4000. Waves that split the rows,
-  // 512 / 1024 / 2048: one tree of 64 over 65537 keys (16 heads on 16 of 96) 84 / 93 / -, 16 ragged int8 trees 126 / 77 / 86.
-  const uint64_t want = wide ? 256 : g.rw == 1 ? (groups > 256 ? 1536 : 1024) : a.sequences == 1 ? 512 : 1024;
+  // them 52.3 / 57.2 / 72.2 us for a token over 27155 keys, 55.7 / 58.8 / 91.5 for 8 x 4000. 
+  // Where the waves split the rows, 512 fill the CUs once, and lengths that the host does not know (several sequences, of
+  // which some are short) need finer parts where a group would have five or fewer. 512 / 1024, f16 and int8: one tree of 64
+  // over 16000 keys (32 heads on 8 of 128) 45.0 / 57.8, 48.7 / 58.6; two over 8000 44.0 / 63.2, 48.0 / 63.4; trees of 32 over 4500
+  // keys, 64 groups 50.9 / 67.1, 52.3 / 65.7, of 4 to 32 over 200 to 4500 41.5 / 44.2, 45.3 / 48.3; 80 groups of these 69.6 / 74.1,
+  // 72.1 / 73.1, ragged 46.2 / 50.2, 51.0 / 54.0; 96 groups 86.2 / 83.6, 91.4 / 84.3, ragged 47.9 / 52.3, 53.4 / 57.3; 104 ragged of 64
+  // 57.2 / 44.4, 62.2 / 61.5; 256 groups, trees of 61 over 4500 130 / 155, 140 / 150, of 5 to 61 over 200 to 4500 112 / 71, 127 / 78. One
+  // prompt chunk of 2048 behind nothing, 512 groups: 88 / 119, 100 / 130; behind 8000 keys 411 / 458, 482 / 526.
+  const bool ragged = a.sequences > 1 && groups >= 96;
+  const uint64_t want = wide ? 256 : g.rw == 1 ? (groups > 256 ? 1536 : 1024) : ragged ? 1024 : 512;
   // A part is two turns of the key waves or more, four 64-key turns where the waves split the rows (one token over 1037
   // keys, one / two / four / eight turns: 9.9 / 8.9 / 10.0 / 11.5 us), and a row has at most 128: with 256 of them a step
   // of 8 rows x 8 heads over 64000 keys takes 65.6 instead of 58.3 us, their join being what grows.
