@@ -437,7 +437,7 @@ ZTVM_API int ztvm_attention(ztvm_ctx* ctx, const ztvm_attention_desc* desc);
  *   logprob[r] = y[tokens[r]] - lse   (a token outside the vocabulary: -inf)
  *   entropy[r] = -sum p ln p, p = exp(y - lse)
  *   top_ids / top_logprobs [r][top_k]: the top_k largest logits in descending order, ties to the lower id, and y - lse of each
- * Any output may be 0 (tokens is read for logprob only). A logit of -inf has probability zero; a row with nothing else
+ * Any output may be 0 (tokens is read for logprob only); an output of one element a row may be tokens itself. A logit of -inf has probability zero; a row with nothing else
  * has log probabilities -inf and entropy 0. A NaN or +inf among the logits makes the row's log probabilities and
  * entropy NaN; the ids still follow the order of the logits, NaN last. */
 typedef struct ztvm_token_logprobs_desc {

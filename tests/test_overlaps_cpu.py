@@ -77,3 +77,10 @@ def test_token_logprobs(capi):
                        (dict(top_ids=0x2004), "tokens"), (dict(top_ids=0x2004, logprob=0), None), (dict(top_logprobs=0x5000), "top_logprobs"),
                        (dict(top_k=0, top_logprobs=0x5000), None), (dict(rows=0, logprob=0x1000), None), (dict(logits_f16=1, logprob=0x1000 + 200), None)]:
         says(capi, "ztvm_token_logprobs", desc(**kw), needle)
+
+
+def test_one_result_a_row_may_replace_the_tokens(capi):
+    base = dict(rows=3, vocab=100, row_stride=100, top_k=1, inv_temperature=1.0, logits=0x1000, tokens=0x8000, logprob=0x9000, entropy=0xA000, top_ids=0xB000)
+    for kw, needle in [(dict(top_ids=0x8000), None), (dict(logprob=0x8000), None), (dict(entropy=0x8000), None), (dict(top_ids=0x8004), "tokens"),
+                       (dict(top_ids=0x8000, top_k=2), "tokens"), (dict(top_ids=0x8000, entropy=0x8000), "top_ids")]:
+        says(capi, "ztvm_token_logprobs", capi.TokenLogprobsDesc(**{**base, **kw}), needle)
