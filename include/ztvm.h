@@ -353,7 +353,8 @@ typedef struct ztvm_kv_cache {
  * Pair j < rotary_dim/2 of a head, elements (j, j + rotary_dim/2) or, interleaved, (2j, 2j+1), is turned by the
  * angle positions[t] * frequencies[j] and scaled by attn_factor; elements from rotary_dim on pass unchanged. The
  * angle is reduced to one turn in 64 bits, so far positions lose nothing; products and sums are f32 and round once
- * to f16. INT8: the f16-rounded row is quantised as ztvm_kv_quantize_int8 does, bit for bit. A slot that is
+ * to f16. INT8: the f16-rounded row is quantised as ztvm_kv_quantize_int8 does, bit for bit (counts are rounded from
+ * x * (1/scale) in f32, so next to a half a count may be one off the quotient's). A slot that is
  * negative or in a page outside the cache stores nothing (its Q row is still written): that is how rows that only
  * pad a batch are marked. Two tokens of one call must not name the same slot. */
 typedef struct ztvm_rope_append_desc {
@@ -407,12 +408,12 @@ ZTVM_API int ztvm_kv_read(ztvm_ctx* ctx, const ztvm_kv_read_desc* desc);
  * Sums are f32, out rounds once to f16. What multiplies the cached values enters that product as f16: the probability, or
  * for INT8 the probability times the value's scale. Each is off by 2^-11 of itself or by 2^-34 of the row's largest,
  * whichever is more (INT8 where more than 32 rows share a kv head: of the largest probability times the scale at hand, which
- * counts as 2^-13 at least). A token that sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds (infinities and NaN among it) does not
- * matter. Rows outside every sequence are left as they were.
+ * counts as 2^-13 at least). A token that sees nothing gives zeros and lse = -inf; what a masked or unwritten slot holds
+ * (infinities and NaN among it) does not matter. Rows outside every sequence are left as they were.
  * max_query and max_kv bound n_b and kv_length[b] (the lengths are read on the device, so a recorded step can be
  * replayed for growing lengths): query tokens past max_query are not written, positions past max_kv not seen (context still
- * goes by kv_length[b]). The work is split over workgroups by these bounds, so bounds near the lengths are the fast ones. Scratch for the joined partial
- * results comes from the context and depends on the descriptor only.
+ * goes by kv_length[b]). The work is split over workgroups by these bounds, so bounds near the lengths are the fast ones.
+ * Scratch for the joined partial results comes from the context and depends on the descriptor only.
  * Head sizes of 32, 64, 96, 128, 160, 192 and 256, page sizes that are multiples of 16 and 16-byte aligned rows run on the matrix
  * cores; everything else is right as well, by a plain kernel. */
 typedef struct ztvm_attention_desc {

@@ -976,9 +976,10 @@ MfmaPlan mfma_plan(const AttentionArgs& a) {
   const uint64_t rows = (uint64_t)a.max_query * group;
   const bool wide = a.cache.head_dim > 128;
   // Few rows: the waves of a workgroup split the keys, so that each key is read by one of them (two waves in flight: a batch
-  // of 48 tokens 160 us, four 164). More: four waves share the staged keys and split the rows, two row tiles each where the
-  // registers hold them (int8 trees of up to 61 x 4 rows: one tile a wave 99 us, two 77; heads of
-  // 256 spill with two: 15 trees of 74 rows over 1846 int8 keys 108 us, with two 158).
+  // of 48 tokens 160 us, four 164). More: four waves share the staged keys and split the rows, two row tiles each up to
+  // heads of 128 (int8 trees of up to 61 x 4 rows: one tile a wave 99 us, two 77, though the int8 instance for heads of 128
+  // fills all 256 registers and spills 8 into its mask branch; heads of 256 spill in the loop: 15 trees of 74 rows over
+  // 1846 int8 keys 108 us, with two 158).
   if (rows <= 16) g.qt = 1, g.rw = 1, g.kw = 2;
   else if (rows <= 32) g.qt = 2, g.rw = 1, g.kw = wide ? 2 : 4;
   else g.qt = rows <= 64 || wide ? 1 : 2, g.rw = 4, g.kw = 1;
