@@ -14,4 +14,9 @@ for (const bad of [-1, 4294967296, 4294967297, 1.5, NaN, Infinity, -Infinity]) {
   assert.throws(call({ cache: Object.assign({}, cache, { page_size: bad }) }), /'page_size' must be a whole number/)
 }
 for (const bad of ['1', true, null, {}]) assert.throws(call({ tokens: bad }), /'tokens' must be a number/)
+for (const fine of [0x4000n, 0x4000]) assert.throws(call({ k_out: fine }), /null context/)
+for (const bad of [-1n, -2n, 1n << 64n, -2, 1.5, NaN, Infinity, 2 ** 53]) {
+  assert.throws(call({ k_out: bad }), /'k_out' must be an address/)
+  assert.throws(call({ cache: Object.assign({}, cache, { pages_capacity: bad }) }), /'pages_capacity' must be an address or a count/)
+}
 console.log('js verify number checks ok')

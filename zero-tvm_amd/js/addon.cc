@@ -611,6 +611,16 @@ bool read_fields(napi_env env, napi_value obj, const Field* fields, size_t n, vo
     napi_get_named_property(env, obj, f.name, &v);
     double number = 0;
     if (f.kind == 'a') {
+      uint64_t whole = 0;
+      bool exact = true, lossless = false;
+      napi_valuetype kind;
+      napi_typeof(env, v, &kind);
+      if (kind == napi_bigint) exact = napi_get_value_bigint_uint64(env, v, &whole, &lossless) == napi_ok && lossless;
+      if (kind == napi_number) exact = napi_get_value_double(env, v, &number) == napi_ok && number >= 0 && number <= 9007199254740991.0 && number == std::floor(number);
+      if (!exact) {
+        napi_throw_range_error(env, nullptr, (std::string("ztvm addon: descriptor field '") + f.name + "' must be an address or a count of 64 bits").c_str());
+        return false;
+      }
       if (!get_u64(env, v, reinterpret_cast<uint64_t*>(at))) return false;
       continue;
     }
